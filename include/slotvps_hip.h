@@ -537,6 +537,60 @@ int svps_slot_attn_f32_fwd(const float* q, const float* k, const float* v, const
 int svps_mask_decode_f32_fwd(const float* feat, const float* embed, const float* bn_scale, const float* bn_shift,
                              float fg_scale, float fg_shift, float* out, int T, int L, int HW, int D, void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Clip-token operators: rotary positions with several axes, attention with its gradient, dense layer with its gradient. The reference
+ * has no counterpart (its slots attend without positions and it ships no training code); they stand beside svps_pos_embed_sine,
+ * svps_slot_self_attn and svps_slot_gemm for 16-bit tokens and for training. `dtype`: SVPS_DTYPE_*. Stride arguments are HOST arrays of
+ * three element strides (batch entry, token, head); the channels of a head are contiguous.
+ *
+ * svps_rotary_axes: y = x with its first R = sum(split) channels turned, R / 2 pairs of channels (j, j + R/2) (pairing 0) or
+ *   (2 j, 2 j + 1) (pairing 1). Pair j belongs to the axis whose section of split[] / 2 pairs it falls into; it turns by
+ *   2 pi turns[j] * pos[.., axis] (inverse: by the negative angle = the gradient). Angles are reduced in float64.
+ *   x [B, N, H, D], optional second tensor x2 [B, N, H2, D] (H2 = 0: none) with the same positions; y / y2 contiguous.
+ *   pos [B or 1 (pos_sb = 0), N, axes], pos_type 0 int32, 1 int64, 2 fp32, strides in elements, axes contiguous, 1 <= axes <= 4.
+ *   split (HOST, even values, sum <= min(D, 256)), turns (HOST, sum / 2 values: frequency / 2 pi). D <= 4096, H + H2 <= 65535.
+ *
+ * svps_attention_fwd: out = softmax(scale q k^T) v over the visible keys, q [B, N, H, D], k / v [B, M, Hk, D], query head h reads key head
+ *   h / (H / Hk); out [B, N, H, D] contiguous, lse [B, H, N] fp32 (NULL: not written) the log-sum-exp of the scaled scores.
+ *   qlens / klens [B] int32 device arrays or NULL (all rows valid), clamped to [0, N] / [0, M]; nothing behind a length is read.
+ *   Visible: frame = 0 every key of the entry; frame > 0: with p = n + klen - qlen, keys j with j / frame <= floor(p / frame), window > 0:
+ *   and more than floor(p / frame) - window. Rows behind qlen and rows that see nothing: out 0, lse -inf.
+ *   D % 8 == 0, D <= 128; scale > 0; tensors aligned to 16 bytes, strides multiples of 8 elements. bf16 / fp16.
+ * svps_attention_bwd: dq, dk, dv (contiguous) from dout and the forward's out (contiguous) and lse, all rows written (zeros where nothing
+ *   flows). Sums in a fixed order: two calls give the same bits.
+ *
+ * svps_linear_act_fwd: y = act(x W^T + bias) + residual; x [M, K] (row stride ldx), W [N, K] (row stride ldw), bias [N] (bias_f32: fp32,
+ *   else of `dtype`; NULL: none), residual [M, N] contiguous or NULL, act 0 none, 1 ReLU, 2 GELU (erf), y [M, N] contiguous, gate [M, N]
+ *   contiguous or NULL: act' at the same place, for the backward call. fp32 sums, one rounding. bf16 / fp16.
+ * svps_linear_act_bwd: dz = dy * gate (gate NULL: dz = dy), dx = dz W, dW = dz^T x, db = column sums of dz; dx / dw / db may be NULL.
+ *   dy [M, N] (row stride ldy), gate contiguous; db fp32 (db_f32) or of `dtype`.
+ * *_workspace_bytes: `unaligned` nonzero if any of the row-strided tensors does not start on 16 bytes. Workspaces start on 16 bytes.
+ * ------------------------------------------------------------------------------------------- */
+#define SVPS_DTYPE_BF16 0
+#define SVPS_DTYPE_F16 1
+#define SVPS_DTYPE_F32 2
+int svps_rotary_axes(const void* x, const long long* sx, void* y, int H, const void* x2, const long long* sx2, void* y2, int H2,
+                     const void* pos, long long pos_sb, long long pos_sn, int pos_type, int axes, const int* split, const double* turns,
+                     int pairing, int inverse, int dtype, int B, int N, int D, void* stream);
+size_t svps_attention_workspace_bytes(int B, int N, int M, int H, int Hk, int D);
+int svps_attention_fwd(const void* q, const long long* sq, const void* k, const long long* sk, const void* v, const long long* sv,
+                       void* out, float* lse, const int* qlens, const int* klens, void* workspace, size_t workspace_bytes, int B, int N,
+                       int M, int H, int Hk, int D, int frame, int window, float scale, int dtype, void* stream);
+size_t svps_attention_bwd_workspace_bytes(int B, int N, int M, int H, int Hk, int D);
+int svps_attention_bwd(const void* dout, const long long* sd, const void* q, const long long* sq, const void* k, const long long* sk,
+                       const void* v, const long long* sv, const void* out, const float* lse, void* dq, void* dk, void* dv,
+                       const int* qlens, const int* klens, void* workspace, size_t workspace_bytes, int B, int N, int M, int H, int Hk,
+                       int D, int frame, int window, float scale, int dtype, void* stream);
+size_t svps_linear_act_workspace_bytes(int M, int K, int N, long long ldx, long long ldw, int unaligned);
+int svps_linear_act_fwd(const void* x, long long ldx, const void* w, long long ldw, const void* bias, int bias_f32, const void* residual,
+                        int act, void* y, void* gate, void* workspace, size_t workspace_bytes, int M, int K, int N, int dtype,
+                        void* stream);
+size_t svps_linear_act_bwd_workspace_bytes(int M, int K, int N, long long ldy, long long ldx, long long ldw, int unaligned, int has_gate,
+                                           int want_dx, int want_dw, int want_db);
+int svps_linear_act_bwd(const void* dy, long long ldy, const void* x, long long ldx, const void* w, long long ldw, const void* gate,
+                        void* dx, void* dw, void* db, int db_f32, void* workspace, size_t workspace_bytes, int M, int K, int N, int dtype,
+                        void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -96,6 +96,15 @@ SIGNATURES = {
     "svps_slot_gemm_f16": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _vp]),
     "svps_slot_gemm_f16_act": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp]),
     "svps_slot_gemm_ln_f16": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _f, _i, _vp, _i, _i, _vp]),
+    "svps_rotary_axes": (_i, [_vp, _vp, _vp, _i, _vp, _vp, _vp, _i, _vp, _c.c_longlong, _c.c_longlong, _i, _i, _vp, _vp] + [_i] * 6 + [_vp]),
+    "svps_attention_workspace_bytes": (_sz, [_i] * 6),
+    "svps_attention_fwd": (_i, [_vp] * 11 + [_sz] + [_i] * 8 + [_f, _i, _vp]),
+    "svps_attention_bwd_workspace_bytes": (_sz, [_i] * 6),
+    "svps_attention_bwd": (_i, [_vp] * 16 + [_sz] + [_i] * 8 + [_f, _i, _vp]),
+    "svps_linear_act_workspace_bytes": (_sz, [_i, _i, _i, _c.c_longlong, _c.c_longlong, _i]),
+    "svps_linear_act_fwd": (_i, [_vp, _c.c_longlong, _vp, _c.c_longlong, _vp, _i, _vp, _i, _vp, _vp, _vp, _sz, _i, _i, _i, _i, _vp]),
+    "svps_linear_act_bwd_workspace_bytes": (_sz, [_i, _i, _i, _c.c_longlong, _c.c_longlong, _c.c_longlong] + [_i] * 5),
+    "svps_linear_act_bwd": (_i, [_vp, _c.c_longlong, _vp, _c.c_longlong, _vp, _c.c_longlong, _vp, _vp, _vp, _vp, _i, _vp, _sz] + [_i] * 4 + [_vp]),
     "svps_set_launch_hook": (None, [_vp]),
     "svps_prof_mark": (None, [_i, _i, _vp]),
 }

@@ -1,0 +1,166 @@
+// Shared by attention_fwd.hip and attention_bwd.hip: attention of 16-bit queries over 16-bit keys and values with shared key heads.
+//
+//   s_ij = scale q_i . k_j for lo_i <= j < hi_i,  p_ij = exp(s_ij - lse_i),  o_i = sum_j p_ij v_j
+//
+// The G = H / Hk query heads of one key head are packed into the row axis: row rr of a (batch entry, key head) pair is token rr / G, head
+// G * hk + rr % G. A tile of rows then reads its keys and values once for all G heads, a single query of G heads is G rows of one tile, and
+// the gradients of a shared head sum inside the matrix products.
+//
+// Visible keys are an interval per row, from lengths and frame order alone (no mask is read): [0, klen) without order; with `frame` > 0
+// tokens of one frame see each other and all earlier frames, `window` > 0 only the last `window` frames, their own counted. The last
+// query stands at the last key. lo and hi never fall along the rows, so tiles outside [lo of the first row, hi of the last) are never
+// visited and only tiles that straddle a bound pay for comparisons.
+//
+// Matrix operands (v_mfma_f32_32x32x16): the scores are computed TRANSPOSED, S^T = K Q^T, so a lane owns one query row and the softmax
+// runs inside the lane (one exchange with lane ^ 32). The accumulator then holds, for a step of 16 keys, keys 4h + {0..3} and 8 + 4h + {0..3}
+// in lane half h; the contraction index of the next product is laid out in that same order (its other operand comes from LDS through the
+// hardware transpose, which takes any row order), so probabilities go from accumulator to operand without crossing lanes.
+//
+// LDS tiles: rows of DP 16-bit channels (DP = head size padded to 32, 64 or 128 with zeros), 16-byte chunk c of row r at position
+// c ^ att_swz(r): fragment reads along a chunk column (16 rows) and transposed reads (4 rows x 4 chunks) both touch 16 different slots.
+#pragma once
+#include "common.h"
+
+namespace svps {
+
+struct AttArgs {
+    const void* q; const void* k; const void* v; const void* dout;
+    void* out;                                  // forward: [B, N, H, D]
+    void* dq; void* dk; void* dv;               // contiguous [B, N, H, D], [B, M, Hk, D]
+    const void* out_in;                         // backward: the forward's output
+    float* lse;                                 // [B, H, N]
+    long long sqb, sqn, sqh, skb, skn, skh, svb, svn, svh, sdb, sdn, sdh;
+    const int* qlens; const int* klens;
+    float* part;                                // partial sums of splits
+    float* stat_lse2; float* stat_delta; int* stat_lo; int* stat_hi;   // backward: per packed row, [B * Hk][rows_pad]
+    int B, N, M, H, Hk, G, D, frame, window, splits, tiles, rows_pad;
+    unsigned gmagic;                            // floor(2^32 / G) + 1
+    float scale;
+};
+
+__device__ __forceinline__ int att_qlen(const AttArgs& a, int b) {
+    if (!a.qlens) return a.N;
+    const int n = a.qlens[b];
+    return n < 0 ? 0 : (n > a.N ? a.N : n);
+}
+__device__ __forceinline__ int att_klen(const AttArgs& a, int b) {
+    if (!a.klens) return a.M;
+    const int n = a.klens[b];
+    return n < 0 ? 0 : (n > a.M ? a.M : n);
+}
+
+// row / G without a division: the product with floor(2^32 / G) + 1 is never short and at most one too far
+__device__ __forceinline__ int att_div_g(const AttArgs& a, int row) {
+    if (a.G == 1) return row;
+    int n = (int)__umulhi((unsigned)row, a.gmagic);
+    return n - ((long long)n * a.G > row ? 1 : 0);
+}
+
+__device__ __forceinline__ int floor_div(int x, int d) {
+    const int q = x / d;
+    return q - ((x - q * d) < 0 ? 1 : 0);
+}
+
+// visible keys [lo, hi) of token n (0 <= n < qlen)
+__device__ __forceinline__ void att_range(const AttArgs& a, int n, int qlen, int klen, int& lo, int& hi) {
+    lo = 0;
+    hi = klen;
+    if (a.frame > 0) {
+        const int p = n + klen - qlen;
+        const int f = a.frame == 1 ? p : floor_div(p, a.frame);
+        const long long end = ((long long)f + 1) * a.frame;
+        hi = end < klen ? (int)end : klen;
+        if (a.window > 0 && f >= a.window) lo = (f - a.window + 1) * a.frame;
+        if (hi < 0) hi = 0;
+        if (lo > hi) lo = hi;
+    }
+}
+
+template <int DP> __device__ __forceinline__ int att_swz(int row) {
+    if constexpr (DP == 128) return ((row & 3) << 2) | ((row >> 2) & 3);
+    else if constexpr (DP == 64) return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
+    else return (row >> 2) & 3;
+}
+
+static __device__ __attribute__((aligned(16))) uint32_t g_att_zero[4];       // never written: the source of padded rows and channels
+
+template <typename T> struct AttVec;
+template <> struct AttVec<__bf16> { typedef bf16x8 v8; typedef bf16x4 v4; };
+template <> struct AttVec<_Float16> { typedef f16x8 v8; typedef f16x4 v4; };
+
+// ROWS rows of a [.., D] matrix into an LDS tile by 16-byte LDS-DMA; `addr(row)` gives a row's global address or null (zeros)
+template <int DP, int ROWS, int NW, typename F>
+__device__ __forceinline__ void att_stage(char* lds, int w, int lane, int D, F addr) {
+    constexpr int CH = DP / 8, RPP = 64 / CH, PIECES = ROWS / RPP;
+#pragma unroll
+    for (int i = 0; i < (PIECES + NW - 1) / NW; ++i) {
+        const int j = i * NW + w;
+        if (PIECES % NW == 0 || j < PIECES) {
+            const int row = j * RPP + lane / CH;
+            const int chunk = (lane % CH) ^ att_swz<DP>(row);
+            const char* p = addr(row);
+            const char* src = (p && chunk * 8 < D) ? p + chunk * 16 : reinterpret_cast<const char*>(g_att_zero);
+            dma16(src, lds + j * 1024);
+        }
+    }
+}
+
+// row fragment: lane (r, h) gets channels 16 ks + 8 h .. + 8 of tile row `row`
+template <typename T, int DP>
+__device__ __forceinline__ typename AttVec<T>::v8 att_row_frag(const char* lds, int row, int ks, int h) {
+    return *reinterpret_cast<const typename AttVec<T>::v8*>(lds + row * (DP * 2) + (((2 * ks + h) ^ att_swz<DP>(row)) << 4));
+}
+
+// transposed fragment: lane (r, h) gets channel 32 db + r of tile rows row0 + 4h + {0..3} and row0 + 8 + 4h + {0..3}
+template <typename T, int DP>
+__device__ __forceinline__ typename AttVec<T>::v8 att_col_frag(const char* lds, int row0, int db, int lane) {
+    typedef typename AttVec<T>::v4 v4;
+    const int g = lane >> 4, i = lane & 15, q = i >> 2, p = i & 3;
+    const int ra = row0 + 4 * (g >> 1) + q, rb = ra + 8;
+    const int chunk = 4 * db + 2 * (g & 1) + (p >> 1);
+    const char* pa = lds + ra * (DP * 2) + ((chunk ^ att_swz<DP>(ra)) << 4) + 8 * (p & 1);
+    const char* pb = lds + rb * (DP * 2) + ((chunk ^ att_swz<DP>(rb)) << 4) + 8 * (p & 1);
+    const v4 lo = ds_tr16((SVPS_LDS v4*)pa);
+    const v4 hi = ds_tr16((SVPS_LDS v4*)pb);
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// eight accumulator values to one operand fragment
+template <typename T>
+__device__ __forceinline__ typename AttVec<T>::v8 att_pack(const float* x) {
+    typename AttVec<T>::v8 r;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) r[j] = (T)x[j];
+    return r;
+}
+
+// a lane's 16 accumulator values of one 32-channel block (channels (i & 3) + 8 (i >> 2) + 4 h) of one row, times f, as 16-bit channels
+template <typename T>
+__device__ __forceinline__ void att_store_block(T* row, int d0, int h, int D, const f32x16& acc, float f) {
+    typedef typename AttVec<T>::v4 v4;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        const int d = d0 + 8 * g + 4 * h;
+        if (d < D) {                                             // D % 8 == 0: a quad is inside or outside as a whole
+            v4 o;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[j] = (T)(acc[4 * g + j] * f);
+            *reinterpret_cast<v4*>(row + d) = o;
+        }
+    }
+}
+
+__device__ __forceinline__ void att_store_block_f32(float* row, int d0, int h, int D, const f32x16& acc) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        const int d = d0 + 8 * g + 4 * h;
+        if (d < D) {
+            f32x4 o;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[j] = acc[4 * g + j];
+            *reinterpret_cast<f32x4*>(row + d) = o;
+        }
+    }
+}
+
+}  // namespace svps

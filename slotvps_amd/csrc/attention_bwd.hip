@@ -1,0 +1,461 @@
+// Attention backward (attention.h has the layouts): the probabilities are computed again from q, k and the forward's log-sum-exp,
+//   p = exp(s - lse),  delta_i = sum_d dO_id O_id,  dV = P^T dO,  dS = P * (dO V^T - delta),  dQ = scale dS K,  dK = scale dS^T Q.
+//
+// Three launches, no atomics, every sum in a fixed order:
+//   att_stats_kernel    per packed row: lse in base 2, delta, visible interval - contiguous, so that the next two read them as vectors
+//   att_dkdv_kernel     a wave owns 32 keys (k, v as operand fragments in registers), walks over the rows that see them (q, dO in LDS)
+//   att_dq_kernel       a wave owns 32 rows, walks over their keys like the forward
+// That is 7 matrix products for the 5 of one joint kernel; the joint form would add dQ from many workgroups with atomics, whose order
+// changes the result, or write every dS to memory (2 bytes per visible pair and head).
+// Few tiles on either side: the walked range is split over workgroups that leave fp32 partial sums, added by att_add_kernel.
+#include "attention.h"
+#include "../../include/slotvps_hip.h"
+
+namespace svps {
+
+// L lanes per packed row, 8 channels each (L * 8 >= D)
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void att_stats_kernel(AttArgs a) {
+    typedef typename AttVec<T>::v8 v8;
+    constexpr int L = DP / 8;
+    const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
+    const int lane = (int)(id % L);
+    const long long prow = id / L;
+    const int pairs = a.B * a.Hk;
+    if (prow >= (long long)pairs * a.rows_pad) return;             // whole groups of L lanes
+    const int pair = (int)(prow / a.rows_pad), row = (int)(prow - (long long)pair * a.rows_pad);
+    const int b = pair / a.Hk, hk = pair - b * a.Hk;
+    const int qlen = att_qlen(a, b), klen = att_klen(a, b);
+    const int n = att_div_g(a, row);
+    const int head = hk * a.G + (row - n * a.G);
+    float s = 0.f;
+    if (n < qlen && 8 * lane < a.D) {
+        const v8 x = *reinterpret_cast<const v8*>((const T*)a.dout + b * a.sdb + n * a.sdn + head * a.sdh + 8 * lane);
+        const v8 y = *reinterpret_cast<const v8*>((const T*)a.out_in + (((long long)b * a.N + n) * a.H + head) * a.D + 8 * lane);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s += (float)x[j] * (float)y[j];
+    }
+#pragma unroll
+    for (int o = 1; o < L; o <<= 1) s += __shfl_xor(s, o);
+    if (lane == 0) {
+        int lo = 0, hi = 0;
+        float lse2 = INFINITY;                                     // exp2(. - inf) = 0: rows behind qlen and rows that see nothing
+        if (n < qlen) {
+            att_range(a, n, qlen, klen, lo, hi);
+            const float x = a.lse[((long long)b * a.H + head) * a.N + n];
+            if (x != -INFINITY) lse2 = x * kLog2e;
+        }
+        a.stat_lse2[prow] = lse2;
+        a.stat_delta[prow] = s;
+        a.stat_lo[prow] = lo;
+        a.stat_hi[prow] = hi;
+    }
+}
+
+template <typename T, int DP, int KT>
+__global__ __launch_bounds__(256, 2) void att_dq_kernel(AttArgs a) {
+    typedef typename AttVec<T>::v8 v8;
+    constexpr int KS = DP / 16, DB = DP / 32, KB = KT / 32, TILE = KT * DP * 2, NW = 4;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int pairs = a.B * a.Hk;
+    const int id = blockIdx.x, pair = id % pairs, rest = id / pairs;
+    const int t = a.tiles - 1 - rest % a.tiles, split = rest / a.tiles;
+    const int b = pair / a.Hk, hk = pair - b * a.Hk;
+    const int qlen = att_qlen(a, b), klen = att_klen(a, b);
+    const int row0 = (t * NW + w) * 32, row = row0 + r;
+    const int n = att_div_g(a, row);
+    const int head = hk * a.G + (row - n * a.G);
+    const bool have = n < qlen;
+    const long long orow = ((long long)b * a.N + n) * a.H + head;
+    const int wg0 = att_div_g(a, t * NW * 32);
+    int wg1 = att_div_g(a, t * NW * 32 + NW * 32 - 1);
+    wg1 = wg1 < qlen ? wg1 : qlen - 1;
+    int tb = 0, te = 0, lo_min = 0, hi_min = 0, lo_max = 0, hi_max = 0, tmp;
+    const int wn0 = att_div_g(a, row0);
+    const bool wave_on = wn0 < qlen;
+    if (wg0 < qlen) {
+        int lo_wg, hi_wg;
+        att_range(a, wg0, qlen, klen, lo_wg, tmp);
+        att_range(a, wg1, qlen, klen, tmp, hi_wg);
+        int wn1 = att_div_g(a, row0 + 31);
+        wn1 = wn1 < qlen ? wn1 : qlen - 1;
+        att_range(a, wave_on ? wn0 : qlen - 1, qlen, klen, lo_min, hi_min);
+        att_range(a, wn1, qlen, klen, lo_max, hi_max);
+        tb = lo_wg / KT;
+        te = hi_wg > lo_wg ? (hi_wg + KT - 1) / KT : tb;
+        if (a.splits > 1) {
+            const int per = (te - tb + a.splits - 1) / a.splits;
+            tb += split * per;
+            te = tb + per < te ? tb + per : te;
+        }
+    }
+    const long long prow = (long long)pair * a.rows_pad + row;     // rows_pad is a multiple of 128
+    const float lse2 = a.stat_lse2[prow], delta = a.stat_delta[prow];
+    const int lo = a.stat_lo[prow], hi = a.stat_hi[prow];
+
+    v8 qf[KS], df[KS];
+    {
+        const T* qp = (const T*)a.q + b * a.sqb + n * a.sqn + head * a.sqh;
+        const T* dp = (const T*)a.dout + b * a.sdb + n * a.sdn + head * a.sdh;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            const int d = 16 * ks + 8 * h;
+            u32x4 x = {0, 0, 0, 0}, y = {0, 0, 0, 0};
+            if (have && d < a.D) {
+                x = *reinterpret_cast<const u32x4*>(qp + d);
+                y = *reinterpret_cast<const u32x4*>(dp + d);
+            }
+            qf[ks] = __builtin_bit_cast(v8, x);
+            df[ks] = __builtin_bit_cast(v8, y);
+        }
+    }
+    const char* kbase = (const char*)((const T*)a.k + b * a.skb + hk * a.skh);
+    const char* vbase = (const char*)((const T*)a.v + b * a.svb + hk * a.svh);
+    auto stage = [&](int tile, int buf) {
+        char* lk = smem + buf * 2 * TILE;
+        const int k0 = tile * KT;
+        att_stage<DP, KT, NW>(lk, w, lane, a.D, [&](int rr) { const int key = k0 + rr; return key < klen ? kbase + (long long)key * a.skn * 2 : nullptr; });
+        att_stage<DP, KT, NW>(lk + TILE, w, lane, a.D, [&](int rr) { const int key = k0 + rr; return key < klen ? vbase + (long long)key * a.svn * 2 : nullptr; });
+    };
+    f32x16 acc[DB];
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[db][i] = 0.f;
+    const float c = a.scale * kLog2e;
+    if (tb < te) stage(tb, 0);
+    for (int tile = tb; tile < te; ++tile) {
+        const int buf = (tile - tb) & 1;
+        wait_vm<0>();
+        wg_barrier();
+        if (tile + 1 < te) stage(tile + 1, buf ^ 1);
+        const int k0 = tile * KT;
+        if (!wave_on || k0 >= hi_max || k0 + KT <= lo_min) continue;
+        const char* lk = smem + buf * 2 * TILE;
+        const char* lv = lk + TILE;
+        const bool whole = k0 >= lo_max && k0 + KT <= hi_min;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+            f32x16 s, dp;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) { s[i] = 0.f; dp[i] = 0.f; }
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                s = mfma16(att_row_frag<T, DP>(lk, 32 * kb + r, ks, h), qf[ks], s);
+                dp = mfma16(att_row_frag<T, DP>(lv, 32 * kb + r, ks, h), df[ks], dp);
+            }
+            float ds[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float p = __builtin_amdgcn_exp2f(fmaf(s[i], c, -lse2));
+                ds[i] = p * (dp[i] - delta);
+            }
+            if (!whole) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int key = k0 + 32 * kb + acc_row(i, h);
+                    if (key < lo || key >= hi) ds[i] = 0.f;
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const v8 pf = att_pack<T>(ds + 8 * u);
+#pragma unroll
+                for (int db = 0; db < DB; ++db) acc[db] = mfma16(att_col_frag<T, DP>(lk, 32 * kb + 16 * u, db, lane), pf, acc[db]);
+            }
+        }
+    }
+    if (n >= a.N) return;
+    if (a.splits > 1) {
+        float* po = a.part + (split * ((long long)a.B * a.N * a.H) + orow) * a.D;
+#pragma unroll
+        for (int db = 0; db < DB; ++db) att_store_block_f32(po, 32 * db, h, a.D, acc[db]);
+        return;
+    }
+    T* o = (T*)a.dq + orow * a.D;
+#pragma unroll
+    for (int db = 0; db < DB; ++db) att_store_block<T>(o, 32 * db, h, a.D, acc[db], a.scale);
+}
+
+template <typename T, int DP, int QT>
+__global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void att_dkdv_kernel(AttArgs a) {
+    typedef typename AttVec<T>::v8 v8;
+    constexpr int KS = DP / 16, DB = DP / 32, QB = QT / 32, TILE = QT * DP * 2, NW = 4;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int pairs = a.B * a.Hk;
+    const int id = blockIdx.x, pair = id % pairs, rest = id / pairs;
+    const int t = rest % a.tiles, split = rest / a.tiles;          // early keys are seen by the most rows: longest first
+    const int b = pair / a.Hk, hk = pair - b * a.Hk;
+    const int qlen = att_qlen(a, b), klen = att_klen(a, b);
+    const int wk0 = t * 32 * NW, k0 = wk0 + 32 * w, key = k0 + r;
+    const bool have = key < klen;
+
+    // tokens that see a key of [wk0, wk1): their frame is not before the first key's, and not `window` or more behind the last key's
+    int n0 = 0, n1 = wk0 < klen ? qlen : 0;
+    if (a.frame > 0 && n1 > 0) {
+        const int wk1 = wk0 + 32 * NW < klen ? wk0 + 32 * NW : klen;
+        const long long off = (long long)klen - qlen;
+        const long long first = (long long)(wk0 / a.frame) * a.frame - off;
+        if (first > 0) n0 = first < qlen ? (int)first : qlen;
+        if (a.window > 0) {
+            const long long last = ((long long)((wk1 - 1) / a.frame) + a.window) * a.frame - off;
+            if (last < n1) n1 = last > 0 ? (int)last : 0;
+        }
+    }
+    int tb = 0, te = 0;
+    if (n0 < n1) {
+        tb = (int)((long long)n0 * a.G / QT);
+        te = (int)(((long long)n1 * a.G + QT - 1) / QT);
+    }
+    if (a.splits > 1) {
+        const int per = (te - tb + a.splits - 1) / a.splits;
+        tb += split * per;
+        te = tb + per < te ? tb + per : te;
+    }
+
+    v8 kf[KS], vf[KS];
+    {
+        const T* kp = (const T*)a.k + b * a.skb + hk * a.skh + (long long)key * a.skn;
+        const T* vp = (const T*)a.v + b * a.svb + hk * a.svh + (long long)key * a.svn;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            const int d = 16 * ks + 8 * h;
+            u32x4 x = {0, 0, 0, 0}, y = {0, 0, 0, 0};
+            if (have && d < a.D) {
+                x = *reinterpret_cast<const u32x4*>(kp + d);
+                y = *reinterpret_cast<const u32x4*>(vp + d);
+            }
+            kf[ks] = __builtin_bit_cast(v8, x);
+            vf[ks] = __builtin_bit_cast(v8, y);
+        }
+    }
+    const char* qbase = (const char*)((const T*)a.q + b * a.sqb + hk * a.G * a.sqh);
+    const char* dbase = (const char*)((const T*)a.dout + b * a.sdb + hk * a.G * a.sdh);
+    auto stage = [&](int tile, int buf) {
+        char* lq = smem + buf * 2 * TILE;
+        auto at = [&](const char* base, long long sn, long long sh, int rr) -> const char* {
+            const int row = tile * QT + rr, n = att_div_g(a, row);
+            return n < qlen ? base + ((long long)n * sn + (long long)(row - n * a.G) * sh) * 2 : nullptr;
+        };
+        att_stage<DP, QT, NW>(lq, w, lane, a.D, [&](int rr) { return at(qbase, a.sqn, a.sqh, rr); });
+        att_stage<DP, QT, NW>(lq + TILE, w, lane, a.D, [&](int rr) { return at(dbase, a.sdn, a.sdh, rr); });
+    };
+    f32x16 dk[DB], dv[DB];
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) { dk[db][i] = 0.f; dv[db][i] = 0.f; }
+    const float c = a.scale * kLog2e;
+    const long long pbase = (long long)pair * a.rows_pad;
+    if (tb < te) stage(tb, 0);
+    for (int tile = tb; tile < te; ++tile) {
+        const int buf = (tile - tb) & 1;
+        wait_vm<0>();
+        wg_barrier();
+        if (tile + 1 < te) stage(tile + 1, buf ^ 1);
+        const char* lq = smem + buf * 2 * TILE;
+        const char* ld = lq + TILE;
+#pragma unroll
+        for (int qb = 0; qb < QB; ++qb) {
+            const int row0 = tile * QT + 32 * qb;
+            const long long pr = pbase + row0;                     // rows_pad is a multiple of 128: in range, padding holds lse2 = inf
+            // interval bounds never fall: first and last row of the block decide whether comparisons are needed, or anything at all
+            const int nlast = att_div_g(a, row0 + 31);
+            const bool tail = nlast >= qlen;
+            const int lo_last = a.stat_lo[pr + 31], hi_first = a.stat_hi[pr], lo_first = a.stat_lo[pr];
+            const bool whole = !tail && k0 >= lo_last && k0 + 32 <= hi_first;
+            if (k0 >= klen || k0 + 32 <= lo_first) continue;
+            f32x16 s, dp;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) { s[i] = 0.f; dp[i] = 0.f; }
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                s = mfma16(att_row_frag<T, DP>(lq, 32 * qb + r, ks, h), kf[ks], s);
+                dp = mfma16(att_row_frag<T, DP>(ld, 32 * qb + r, ks, h), vf[ks], dp);
+            }
+            float p[16], ds[16];
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const f32x4 ls = *reinterpret_cast<const f32x4*>(a.stat_lse2 + pr + 8 * g + 4 * h);
+                const f32x4 de = *reinterpret_cast<const f32x4*>(a.stat_delta + pr + 8 * g + 4 * h);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int i = 4 * g + j;
+                    p[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, -ls[j]));
+                    ds[i] = p[i] * (dp[i] - de[j]);
+                }
+            }
+            if (!whole) {
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    typedef int i32x4 __attribute__((ext_vector_type(4)));
+                    const i32x4 lo = *reinterpret_cast<const i32x4*>(a.stat_lo + pr + 8 * g + 4 * h);
+                    const i32x4 hi = *reinterpret_cast<const i32x4*>(a.stat_hi + pr + 8 * g + 4 * h);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (key < lo[j] || key >= hi[j]) { p[4 * g + j] = 0.f; ds[4 * g + j] = 0.f; }
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const v8 pf = att_pack<T>(p + 8 * u), sf = att_pack<T>(ds + 8 * u);
+#pragma unroll
+                for (int db = 0; db < DB; ++db) {
+                    dv[db] = mfma16(att_col_frag<T, DP>(ld, 32 * qb + 16 * u, db, lane), pf, dv[db]);
+                    dk[db] = mfma16(att_col_frag<T, DP>(lq, 32 * qb + 16 * u, db, lane), sf, dk[db]);
+                }
+            }
+        }
+    }
+    if (key >= a.M) return;
+    const long long orow = ((long long)b * a.M + key) * a.Hk + hk;
+    if (a.splits > 1) {
+        const long long rows = (long long)a.B * a.M * a.Hk;
+        float* pk = a.part + (split * rows + orow) * a.D;
+        float* pv = pk + (long long)a.splits * rows * a.D;
+#pragma unroll
+        for (int db = 0; db < DB; ++db) {
+            att_store_block_f32(pk, 32 * db, h, a.D, dk[db]);
+            att_store_block_f32(pv, 32 * db, h, a.D, dv[db]);
+        }
+        return;
+    }
+    T* ok = (T*)a.dk + orow * a.D;
+    T* ov = (T*)a.dv + orow * a.D;
+#pragma unroll
+    for (int db = 0; db < DB; ++db) {
+        att_store_block<T>(ok, 32 * db, h, a.D, dk[db], a.scale);
+        att_store_block<T>(ov, 32 * db, h, a.D, dv[db], 1.f);
+    }
+}
+
+// out = f * sum over splits, four values per thread, splits in order (count % 4 == 0: D % 8 == 0)
+template <typename T>
+__global__ __launch_bounds__(256) void att_add_kernel(const float* part, T* out, long long count, int splits, float f) {
+    const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (i >= count) return;
+    f32x4 s = {0.f, 0.f, 0.f, 0.f};
+    for (int k = 0; k < splits; ++k) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(part + k * count + i);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[j] += x[j];
+    }
+    typename AttVec<T>::v4 o;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[j] = (T)(s[j] * f);
+    *reinterpret_cast<typename AttVec<T>::v4*>(out + i) = o;
+}
+
+int attention_check(const void* const* ptrs, int np, const long long* const* strides, int ns, int B, int N, int M, int H, int Hk, int D,
+                    int frame, int window, float scale, int dtype);
+
+struct AttBwdPlan {
+    int q_tiles, q_splits, k_tiles, k_splits, rows_pad;
+    size_t stat_bytes, part_bytes;
+};
+
+static AttBwdPlan attention_bwd_plan(int B, int N, int M, int H, int Hk, int D) {
+    AttBwdPlan p;
+    const long long rows = (long long)N * (H / Hk), pairs = (long long)B * Hk, want = 2LL * svps_num_cus();
+    p.q_tiles = (int)((rows + 127) / 128);
+    p.k_tiles = (M + 127) / 128;
+    p.rows_pad = p.q_tiles * 128;
+    auto pick = [&](long long wgs, long long steps) {
+        long long s = wgs * 2 > want ? 1 : want / wgs;
+        if (s > steps / 4) s = steps / 4;
+        if (s > 32) s = 32;
+        return s < 1 ? 1 : (int)s;
+    };
+    p.q_splits = pick(pairs * p.q_tiles, (M + 63) / 64);
+    p.k_splits = pick(pairs * p.k_tiles, (rows + 63) / 64);
+    p.stat_bytes = (size_t)pairs * p.rows_pad * 4 * sizeof(float);
+    const size_t a = p.q_splits > 1 ? (size_t)p.q_splits * B * N * H * D * sizeof(float) : 0;
+    const size_t c = p.k_splits > 1 ? (size_t)p.k_splits * B * M * Hk * D * 2 * sizeof(float) : 0;
+    p.part_bytes = a > c ? a : c;                                  // one after the other on one stream: shared
+    return p;
+}
+
+template <typename T, int DP>
+static int attention_bwd_launch(AttArgs a, const AttBwdPlan& p, hipStream_t stream) {
+    static SvpsLdsAttr attr_q, attr_k;
+    constexpr int KT = 64, QT = 64, LDS = 4 * 64 * DP * 2;
+    hipError_t e = attr_q.ensure((const void*)att_dq_kernel<T, DP, KT>, LDS);
+    if (e == hipSuccess) e = attr_k.ensure((const void*)att_dkdv_kernel<T, DP, QT>, LDS);
+    if (e != hipSuccess) return (int)e;
+    const long long pairs = (long long)a.B * a.Hk;
+    const long long lanes = pairs * a.rows_pad * (DP / 8);
+    hipLaunchKernelGGL((att_stats_kernel<T, DP>), dim3((unsigned)((lanes + 255) / 256)), dim3(256), 0, stream, a);
+    e = hipGetLastError();
+    if (e != hipSuccess) return (int)e;
+    AttArgs k = a;
+    k.tiles = p.k_tiles;
+    k.splits = p.k_splits;
+    hipLaunchKernelGGL((att_dkdv_kernel<T, DP, QT>), dim3((unsigned)(pairs * k.tiles * k.splits)), dim3(256), LDS, stream, k);
+    e = hipGetLastError();
+    if (e != hipSuccess) return (int)e;
+    if (k.splits > 1) {
+        const long long count = (long long)a.B * a.M * a.Hk * a.D;
+        const unsigned grid = (unsigned)((count / 4 + 255) / 256);
+        hipLaunchKernelGGL(att_add_kernel<T>, dim3(grid), dim3(256), 0, stream, a.part, (T*)a.dk, count, k.splits, a.scale);
+        hipLaunchKernelGGL(att_add_kernel<T>, dim3(grid), dim3(256), 0, stream, a.part + k.splits * count, (T*)a.dv, count, k.splits, 1.f);
+        e = hipGetLastError();
+        if (e != hipSuccess) return (int)e;
+    }
+    AttArgs q = a;
+    q.tiles = p.q_tiles;
+    q.splits = p.q_splits;
+    hipLaunchKernelGGL((att_dq_kernel<T, DP, KT>), dim3((unsigned)(pairs * q.tiles * q.splits)), dim3(256), LDS, stream, q);
+    e = hipGetLastError();
+    if (e != hipSuccess) return (int)e;
+    if (q.splits > 1) {
+        const long long count = (long long)a.B * a.N * a.H * a.D;
+        hipLaunchKernelGGL(att_add_kernel<T>, dim3((unsigned)((count / 4 + 255) / 256)), dim3(256), 0, stream, a.part, (T*)a.dq, count, q.splits, a.scale);
+        e = hipGetLastError();
+    }
+    return (int)e;
+}
+
+}  // namespace svps
+
+extern "C" size_t svps_attention_bwd_workspace_bytes(int B, int N, int M, int H, int Hk, int D) {
+    if (B <= 0 || N <= 0 || M <= 0 || H <= 0 || Hk <= 0 || H % Hk || D <= 0) return 0;
+    const svps::AttBwdPlan p = svps::attention_bwd_plan(B, N, M, H, Hk, D);
+    return p.stat_bytes + p.part_bytes;
+}
+
+extern "C" int svps_attention_bwd(const void* dout, const long long* sd, const void* q, const long long* sq, const void* k, const long long* sk,
+                                  const void* v, const long long* sv, const void* out, const float* lse, void* dq, void* dk, void* dv,
+                                  const int* qlens, const int* klens, void* workspace, size_t workspace_bytes, int B, int N, int M, int H,
+                                  int Hk, int D, int frame, int window, float scale, int dtype, void* stream) {
+    using namespace svps;
+    const void* ptrs[] = {dout, q, k, v, out, dq, dk, dv, workspace};
+    const long long* st[] = {sd, sq, sk, sv};
+    if (!lse) return SVPS_ERR_BAD_ARG;
+    const int rc = attention_check(ptrs, 9, st, 4, B, N, M, H, Hk, D, frame, window, scale, dtype);
+    if (rc) return rc;
+    const AttBwdPlan p = attention_bwd_plan(B, N, M, H, Hk, D);
+    if (workspace_bytes < p.stat_bytes + p.part_bytes) return SVPS_ERR_WORKSPACE;
+    AttArgs a = {};
+    a.q = q; a.k = k; a.v = v; a.dout = dout; a.out_in = out; a.lse = const_cast<float*>(lse);
+    a.dq = dq; a.dk = dk; a.dv = dv; a.qlens = qlens; a.klens = klens;
+    a.sqb = sq[0]; a.sqn = sq[1]; a.sqh = sq[2]; a.skb = sk[0]; a.skn = sk[1]; a.skh = sk[2];
+    a.svb = sv[0]; a.svn = sv[1]; a.svh = sv[2]; a.sdb = sd[0]; a.sdn = sd[1]; a.sdh = sd[2];
+    const size_t rows = (size_t)B * Hk * p.rows_pad;
+    a.stat_lse2 = (float*)workspace;
+    a.stat_delta = a.stat_lse2 + rows;
+    a.stat_lo = (int*)(a.stat_delta + rows);
+    a.stat_hi = a.stat_lo + rows;
+    a.part = (float*)((char*)workspace + p.stat_bytes);
+    a.rows_pad = p.rows_pad;
+    a.B = B; a.N = N; a.M = M; a.H = H; a.Hk = Hk; a.G = H / Hk; a.D = D; a.frame = frame; a.window = window;
+    a.scale = scale;
+    a.gmagic = a.G > 1 ? (unsigned)(0x100000000ULL / a.G) + 1 : 0;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    if (dtype == SVPS_DTYPE_BF16)
+        return D <= 32 ? attention_bwd_launch<__bf16, 32>(a, p, s) : D <= 64 ? attention_bwd_launch<__bf16, 64>(a, p, s) : attention_bwd_launch<__bf16, 128>(a, p, s);
+    return D <= 32 ? attention_bwd_launch<_Float16, 32>(a, p, s) : D <= 64 ? attention_bwd_launch<_Float16, 64>(a, p, s) : attention_bwd_launch<_Float16, 128>(a, p, s);
+}

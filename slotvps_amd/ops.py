@@ -5,6 +5,8 @@ PyTorch is used for device memory and the current stream only. Every function re
 restatement used for checking lives in oracle/ and is never imported from this package.
 """
 import ctypes
+import functools
+import math
 
 import torch
 
@@ -1113,6 +1115,398 @@ def mask_decode_f32(feat, embed, bn_scale, bn_shift, fg_scale, fg_shift):
                                           float(fg_shift), _ptr(out), T, L, HW, D, ctx.stream)
     _lib.check(rc, "svps_mask_decode_f32_fwd")
     return out
+
+
+# ---- clip-token operators for 16-bit tokens and for training: rotary positions with several axes (csrc/rotary_axes.hip), attention with
+# ---- its gradient (csrc/attention_fwd.hip, attention_bwd.hip), dense layer with its gradient (csrc/linear_act.hip). rotary_axes, attention
+# ---- and linear_act are differentiable; the *_bwd functions are the same gradients as plain calls (no autograd graph), the form to
+# ---- capture: inside a HIP graph capture the autograd backward of these three is refused.
+
+_DTYPE_CODE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_POS_CODE = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
+_LL3 = ctypes.c_longlong * 3
+
+
+def _token_tensor(t, name, dtypes):
+    """GPU tensor of one of `dtypes` with contiguous channels (anything else of that kind is copied)."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise RuntimeError(f"{name}: GPU tensors only (got {'a non-tensor' if not isinstance(t, torch.Tensor) else t.device}); "
+                           "there is no CPU fallback")
+    if t.dtype not in dtypes:
+        raise TypeError(f"{name}: expected one of {', '.join(str(d) for d in dtypes)}, got {t.dtype}")
+    return t if t.dim() == 0 or t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _no_capture(what):
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError(f"{what}: the autograd backward inside a graph capture is refused - gradients of leaves that an eager graph still "
+                           f"holds would be accumulated on that graph's stream, which ends the capture and the process; capture ops.{what}_bwd")
+
+
+@functools.lru_cache(maxsize=64)
+def _rotary_table(split, base, ladder):
+    """(int array of split, double array of frequency / (2 pi) per pair): the frequency of pair i of a section of d channels is
+    base^(-2 i / d) (ladder "axis": every axis starts at 1) or, with j counting through all sections, base^(-2 j / sum) ("shared")."""
+    total = sum(split)
+    turns = []
+    for d in split:
+        for i in range(d // 2):
+            e = 2.0 * i / d if ladder == "axis" else 2.0 * len(turns) / total
+            turns.append(float(base) ** -e / (2.0 * math.pi))
+    return (ctypes.c_int * len(split))(*split), (ctypes.c_double * len(turns))(*turns)
+
+
+def _rotary_args(x, positions, split, base, pairing, ladder, also):
+    split = tuple(int(d) for d in split)
+    if not 1 <= len(split) <= 4 or any(d < 2 or d % 2 for d in split):
+        raise ValueError(f"rotary_axes: split must be one to four even channel counts, got {split}")
+    if pairing not in ("half", "adjacent") or ladder not in ("axis", "shared"):
+        raise ValueError("rotary_axes: pairing is 'half' or 'adjacent', ladder is 'axis' or 'shared'")
+    if not (base > 0.0 and math.isfinite(base)):
+        raise ValueError("rotary_axes: base must be a positive number")
+    x = _token_tensor(x, "x", _DTYPE_CODE)
+    if x.dim() != 4:
+        raise ValueError(f"rotary_axes: x is [B, N, H, D], got {tuple(x.shape)}")
+    B, N, _, D = x.shape
+    if sum(split) > min(D, 256):
+        raise ValueError(f"rotary_axes: split {split} needs more than the {min(D, 256)} channels that can turn")
+    if D > 4096:
+        raise ValueError("rotary_axes: at most 4096 channels per head")
+    if also is not None:
+        also = _token_tensor(also, "also", (x.dtype,))
+        if also.dim() != 4 or also.shape[:2] != x.shape[:2] or also.shape[3] != D:
+            raise ValueError(f"rotary_axes: also is [B, N, H2, D] with x's B, N, D, got {tuple(also.shape)} beside {tuple(x.shape)}")
+    positions = _token_tensor(positions, "positions", _POS_CODE)
+    A = len(split)
+    if positions.shape != (N, A) and positions.shape != (B, N, A):
+        raise ValueError(f"rotary_axes: positions must be [{N}, {A}] or [{B}, {N}, {A}], got {tuple(positions.shape)}")
+    if x.shape[2] + (also.shape[2] if also is not None else 0) > 65535:
+        raise ValueError("rotary_axes: more than 65535 heads")
+    return x, positions, split, also
+
+
+def _rotary_launch(x, positions, split, base, pairing, ladder, also, inverse):
+    B, N, H, D = x.shape
+    y = torch.empty((B, N, H, D), dtype=x.dtype, device=x.device)
+    y2 = None if also is None else torch.empty(also.shape, dtype=x.dtype, device=x.device)
+    if also is not None and also.shape[2] == 0:
+        also = None
+    if H == 0 and also is not None:                              # the launch needs a first tensor with heads
+        y2.copy_(_rotary_launch(also, positions, split, base, pairing, ladder, None, inverse)[0])
+        return y, y2
+    if B == 0 or N == 0 or H == 0:
+        return y, y2
+    lib = _lib.load()
+    csplit, turns = _rotary_table(split, float(base), ladder)
+    ps = positions.stride()
+    psb, psn = (0, ps[0]) if positions.dim() == 2 else (ps[0], ps[1])
+    with _on(x, positions, also, y, y2) as ctx:
+        rc = lib.svps_rotary_axes(x.data_ptr(), _LL3(*x.stride()[:3]), y.data_ptr(), H,
+                                  None if also is None else also.data_ptr(), None if also is None else _LL3(*also.stride()[:3]),
+                                  None if also is None else y2.data_ptr(), 0 if also is None else also.shape[2],
+                                  positions.data_ptr(), psb, psn, _POS_CODE[positions.dtype], len(split), csplit, turns,
+                                  0 if pairing == "half" else 1, int(inverse), _DTYPE_CODE[x.dtype], B, N, D, ctx.stream)
+    _lib.check(rc, "svps_rotary_axes")
+    return y, y2
+
+
+class _RotaryAxes(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, also, positions, cfg):
+        ctx.save_for_backward(positions)
+        ctx.cfg, ctx.two = cfg, also is not None
+        y, y2 = _rotary_launch(x, positions, *cfg, also, False)
+        return (y, y2) if also is not None else y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dy2=None):
+        _no_capture("rotary_axes")
+        positions, = ctx.saved_tensors
+        fix = lambda t: _token_tensor(t, "dy", _DTYPE_CODE)
+        dx, dx2 = _rotary_launch(fix(dy), positions, *ctx.cfg, fix(dy2) if ctx.two else None, True)
+        return dx, dx2, None, None
+
+
+def rotary_axes(x, positions, split, base=10000.0, pairing="half", ladder="axis", also=None):
+    """Rotary positions with several axes, e.g. (frame, row, column) of a clip's tokens. x [B, N, H, D] (fp32 / bf16 / fp16, any strides
+    with contiguous channels); positions [N, A] or [B, N, A] (int32, int64 or fp32), A = len(split) <= 4 axes; split: even channel counts per
+    axis, their sum R <= D channels turn, the others pass. Pair j of the R / 2 pairs is channels (j, j + R/2) (pairing "half") or
+    (2 j, 2 j + 1) ("adjacent") and turns by position * frequency: base^(-2 i / d) along each axis' own d channels (ladder "axis") or
+    base^(-2 j / R) through all of them ("shared"). Angles are reduced in float64: far positions keep theirs.
+    also: a second tensor [B, N, H2, D] of x's dtype (the keys beside the queries), turned in the same launch -> (y, y2); else y.
+    Outputs are contiguous. Differentiable in x and also."""
+    x, positions, split, also = _rotary_args(x, positions, split, base, pairing, ladder, also)
+    cfg = (split, float(base), pairing, ladder)
+    if torch.is_grad_enabled() and (x.requires_grad or (also is not None and also.requires_grad)):
+        return _RotaryAxes.apply(x, also, positions, cfg)
+    y, y2 = _rotary_launch(x, positions, *cfg, also, False)
+    return y if also is None else (y, y2)
+
+
+def rotary_axes_bwd(dy, positions, split, base=10000.0, pairing="half", ladder="axis", also=None):
+    """Gradient of rotary_axes as a plain call: the rotation by the negative angles. Arguments as there, dy (and also: dy2) in x's place."""
+    dy, positions, split, also = _rotary_args(dy, positions, split, base, pairing, ladder, also)
+    dx, dx2 = _rotary_launch(dy, positions, split, float(base), pairing, ladder, also, True)
+    return dx if also is None else (dx, dx2)
+
+
+_TOKENS16 = (torch.bfloat16, torch.float16)
+
+
+def _att_tensor(t, name, dtype=None):
+    """16-byte rows for the attention kernels: channels contiguous, strides multiples of 8, base aligned; otherwise a copy."""
+    t = _token_tensor(t, name, _TOKENS16 if dtype is None else (dtype,))
+    if t.dim() != 4:
+        raise ValueError(f"attention: {name} must have 4 dims [batch, tokens, heads, channels], got {tuple(t.shape)}")
+    s = t.stride()
+    if (t.data_ptr() & 15) or any((s[i] & 7) and t.shape[i] > 1 for i in range(3)):
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _att_strides(t):
+    s, n = t.stride(), t.shape
+    return _LL3(s[0] if n[0] > 1 else 0, s[1] if n[1] > 1 else 0, s[2] if n[2] > 1 else 0)
+
+
+def _att_args(q, k, v, q_lens, k_lens, frame, window, scale):
+    q = _att_tensor(q, "q")
+    k, v = _att_tensor(k, "k", q.dtype), _att_tensor(v, "v", q.dtype)
+    B, N, H, D = q.shape
+    M, Hk = k.shape[1], k.shape[2]
+    if k.shape != (B, M, Hk, D) or v.shape != k.shape:
+        raise ValueError(f"attention: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} do not match ([B, N, H, D] and twice [B, M, Hk, D])")
+    if H < 1 or Hk < 1 or H % Hk:
+        raise ValueError(f"attention: {H} query heads over {Hk} key heads (a multiple is needed)")
+    if D % 8 or not 8 <= D <= 128:
+        raise ValueError(f"attention: head size {D} (a multiple of 8 up to 128 is needed)")
+    frame, window = int(frame), int(window)
+    if frame < 0 or window < 0 or frame > 1 << 30 or window > 1 << 30 or (window and not frame):
+        raise ValueError("attention: frame and window must not be negative, and a window needs a frame size")
+    scale = D ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale <= 1e30:
+        raise ValueError("attention: scale must be positive")
+    for name, t in (("q_lens", q_lens), ("k_lens", k_lens)):
+        if t is not None:
+            _need(t, name, torch.int32, 1)
+            if t.shape[0] != B:
+                raise ValueError(f"attention: {name} needs one length per batch entry")
+    return q, k, v, (q_lens, k_lens, frame, window, scale)
+
+
+def _att_fwd(q, k, v, q_lens, k_lens, frame, window, scale, want_lse):
+    B, N, H, D = q.shape
+    M, Hk = k.shape[1], k.shape[2]
+    empty = B == 0 or N == 0 or M == 0
+    out = (torch.zeros if empty else torch.empty)((B, N, H, D), dtype=q.dtype, device=q.device)
+    lse = torch.empty((B, H, N), dtype=torch.float32, device=q.device) if want_lse else None
+    if empty:
+        if lse is not None:
+            lse.fill_(float("-inf"))
+        return out, lse
+    lib = _lib.load()
+    with _on(q, k, v, out, lse, q_lens, k_lens) as ctx:
+        nbytes = lib.svps_attention_workspace_bytes(B, N, M, H, Hk, D)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+        rc = lib.svps_attention_fwd(q.data_ptr(), _att_strides(q), k.data_ptr(), _att_strides(k), v.data_ptr(), _att_strides(v),
+                                    out.data_ptr(), _ptr(lse), _ptr(q_lens), _ptr(k_lens), _ptr(ws), nbytes, B, N, M, H, Hk, D,
+                                    frame, window, scale, _DTYPE_CODE[q.dtype], ctx.stream)
+    _lib.check(rc, "svps_attention_fwd")
+    return out, lse
+
+
+def _att_bwd(dout, q, k, v, out, lse, q_lens, k_lens, frame, window, scale):
+    B, N, H, D = q.shape
+    M, Hk = k.shape[1], k.shape[2]
+    dout = _att_tensor(dout, "dout", q.dtype)
+    out = _att_tensor(out, "out", q.dtype).contiguous()
+    _need(lse, "lse", torch.float32, 3)
+    if dout.shape != q.shape or out.shape != q.shape or lse.shape != (B, H, N):
+        raise ValueError(f"attention_bwd: dout {tuple(dout.shape)}, out {tuple(out.shape)}, lse {tuple(lse.shape)} do not belong to q {tuple(q.shape)}")
+    empty = B == 0 or N == 0 or M == 0
+    new = torch.zeros if empty else torch.empty
+    dq = new((B, N, H, D), dtype=q.dtype, device=q.device)
+    dk = new((B, M, Hk, D), dtype=q.dtype, device=q.device)
+    dv = new((B, M, Hk, D), dtype=q.dtype, device=q.device)
+    if empty:
+        return dq, dk, dv
+    lib = _lib.load()
+    with _on(dout, q, k, v, out, lse, q_lens, k_lens) as ctx:
+        nbytes = lib.svps_attention_bwd_workspace_bytes(B, N, M, H, Hk, D)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        rc = lib.svps_attention_bwd(dout.data_ptr(), _att_strides(dout), q.data_ptr(), _att_strides(q), k.data_ptr(), _att_strides(k),
+                                    v.data_ptr(), _att_strides(v), out.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                                    _ptr(q_lens), _ptr(k_lens), ws.data_ptr(), nbytes, B, N, M, H, Hk, D, frame, window, scale,
+                                    _DTYPE_CODE[q.dtype], ctx.stream)
+    _lib.check(rc, "svps_attention_bwd")
+    return dq, dk, dv
+
+
+class _Attention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, q_lens, k_lens, frame, window, scale):
+        out, lse = _att_fwd(q, k, v, q_lens, k_lens, frame, window, scale, True)
+        ctx.save_for_backward(q, k, v, out, lse, q_lens, k_lens)
+        ctx.cfg = (frame, window, scale)
+        ctx.mark_non_differentiable(lse)
+        return out, lse
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout, _):
+        _no_capture("attention")
+        q, k, v, out, lse, q_lens, k_lens = ctx.saved_tensors
+        return (*_att_bwd(dout, q, k, v, out, lse, q_lens, k_lens, *ctx.cfg), None, None, None, None, None)
+
+
+def attention(q, k, v, q_lens=None, k_lens=None, frame=0, window=0, scale=None, return_lse=False):
+    """softmax(scale q k^T) v for 16-bit tokens (bf16 / fp16): q [B, N, H, D], k / v [B, M, Hk, D] (views are fine: contiguous channels,
+    other strides multiples of 8 elements, 16-byte aligned - anything else is copied first); query head h reads key head h // (H / Hk);
+    D a multiple of 8 up to 128; scale defaults to D^-0.5.
+    q_lens / k_lens [B] int32 (on the GPU, clamped to [0, N] / [0, M]): tokens behind them do not take part and may hold anything.
+    frame = 0: every query sees every key. frame > 0: tokens of one frame (that many tokens) see each other and all earlier frames (1: the
+    causal order of single tokens), window > 0: only the last `window` frames with their own. The last query stands at the last key, so N
+    new tokens attend over a memory of M >= N with the same arguments. Keys that a row does not see but that lie within its batch entry's
+    length must be finite.
+    Returns out [B, N, H, D] (zeros for rows behind q_lens and rows that see nothing); with return_lse also the log-sum-exp [B, H, N] fp32
+    (-inf for such rows) that attention_bwd takes. Differentiable in q, k, v. Single queries over a long memory are split over its keys."""
+    q, k, v, cfg = _att_args(q, k, v, q_lens, k_lens, frame, window, scale)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        out, lse = _Attention.apply(q, k, v, *cfg)
+    else:
+        out, lse = _att_fwd(q, k, v, *cfg, return_lse)
+    return (out, lse) if return_lse else out
+
+
+def attention_bwd(dout, q, k, v, out, lse, q_lens=None, k_lens=None, frame=0, window=0, scale=None):
+    """Gradients (dq, dk, dv) of attention as a plain call, from the forward's out and lse and the same other arguments. The probabilities
+    are computed again; sums run in a fixed order (two calls give the same bits). Rows and keys behind the lengths get zeros."""
+    q, k, v, cfg = _att_args(q, k, v, q_lens, k_lens, frame, window, scale)
+    return _att_bwd(dout, q, k, v, out, lse, *cfg)
+
+
+def _rows16(t, name, dtype, cols):
+    """[..., cols] -> 2-D rows with contiguous columns and a row stride >= cols (a view where that is possible)."""
+    t = _token_tensor(t, name, (dtype,))
+    t = t.reshape(-1, cols)
+    if (cols > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < cols):
+        t = t.contiguous()
+    return t
+
+
+def _ld(t):
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _linear_args(x, weight, bias, act, residual):
+    x = _token_tensor(x, "x", _TOKENS16)
+    if not isinstance(weight, torch.Tensor) or weight.dim() != 2 or x.dim() < 1:
+        raise ValueError("linear_act: x is [..., K], weight [N, K]")
+    N, K = weight.shape
+    if x.shape[-1] != K or K == 0:
+        raise ValueError(f"linear_act: x {tuple(x.shape)} does not match weight {tuple(weight.shape)}")
+    weight = _rows16(weight, "weight", x.dtype, K)
+    if act not in (ACT_NONE, ACT_RELU, ACT_GELU):
+        raise ValueError("linear_act: act must be ACT_NONE, ACT_RELU or ACT_GELU")
+    if bias is not None:
+        if not isinstance(bias, torch.Tensor) or bias.dtype not in (x.dtype, torch.float32):
+            raise TypeError(f"bias: expected {x.dtype} or torch.float32")
+        _need(bias, "bias", bias.dtype, 1)
+        if bias.shape[0] != N:
+            raise ValueError(f"linear_act: bias must have {N} values")
+    if residual is not None:
+        residual = _token_tensor(residual, "residual", (x.dtype,))
+        if residual.shape != x.shape[:-1] + (N,):
+            raise ValueError(f"linear_act: residual must be {tuple(x.shape[:-1]) + (N,)}, got {tuple(residual.shape)}")
+        residual = residual.contiguous()
+    return x, weight, residual
+
+
+def _linear_fwd(x, weight, bias, act, residual, want_gate):
+    N, K = weight.shape
+    shape = x.shape[:-1] + (N,)
+    y = torch.empty(shape, dtype=x.dtype, device=x.device)
+    gate = torch.empty(shape, dtype=x.dtype, device=x.device) if want_gate and act != ACT_NONE else None
+    x2 = _rows16(x, "x", x.dtype, K) if x.numel() else x
+    M = y.numel() // N if N else 0
+    if M == 0:
+        return y, gate
+    lib = _lib.load()
+    with _on(x, weight, bias, residual, y) as ctx:
+        ldx, ldw = _ld(x2), _ld(weight)
+        nbytes = lib.svps_linear_act_workspace_bytes(M, K, N, ldx, ldw, (x2.data_ptr() | weight.data_ptr()) & 15)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+        rc = lib.svps_linear_act_fwd(x2.data_ptr(), ldx, weight.data_ptr(), ldw, _ptr(bias), int(bias is not None and bias.dtype == torch.float32),
+                                     _ptr(residual), int(act), y.data_ptr(), _ptr(gate), _ptr(ws), nbytes, M, K, N, _DTYPE_CODE[x.dtype], ctx.stream)
+    _lib.check(rc, "svps_linear_act_fwd")
+    return y, gate
+
+
+def _linear_bwd(dy, x, weight, gate, bias, want_dx, want_dw):
+    N, K = weight.shape
+    if dy.shape != x.shape[:-1] + (N,) or (gate is not None and gate.shape != dy.shape):
+        raise ValueError(f"linear_act_bwd: dy {tuple(dy.shape)} (and gate) do not belong to x {tuple(x.shape)} and weight {tuple(weight.shape)}")
+    empty = dy.numel() == 0
+    new = torch.zeros if empty else torch.empty
+    dx = new(x.shape, dtype=x.dtype, device=x.device) if want_dx else None
+    dw = new((N, K), dtype=x.dtype, device=x.device) if want_dw else None
+    db = new((N,), dtype=bias.dtype, device=x.device) if bias is not None else None
+    if empty or not (want_dx or want_dw or bias is not None):
+        return dx, dw, db
+    x2, dy2 = _rows16(x, "x", x.dtype, K), _rows16(dy, "dy", x.dtype, N)
+    M = dy2.shape[0]
+    lib = _lib.load()
+    with _on(dy, x, weight, gate, bias) as ctx:
+        ldy, ldx, ldw = _ld(dy2), _ld(x2), _ld(weight)
+        nbytes = lib.svps_linear_act_bwd_workspace_bytes(M, K, N, ldy, ldx, ldw, (x2.data_ptr() | weight.data_ptr() | dy2.data_ptr()) & 15,
+                                                         int(gate is not None), int(want_dx), int(want_dw), int(db is not None))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+        rc = lib.svps_linear_act_bwd(dy2.data_ptr(), ldy, x2.data_ptr(), ldx, weight.data_ptr(), ldw, _ptr(gate), _ptr(dx), _ptr(dw), _ptr(db),
+                                     int(db is not None and db.dtype == torch.float32), _ptr(ws), nbytes, M, K, N, _DTYPE_CODE[x.dtype], ctx.stream)
+    _lib.check(rc, "svps_linear_act_bwd")
+    return dx, dw, db
+
+
+class _LinearAct(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, act):
+        y, gate = _linear_fwd(x, weight, bias, act, residual, any(ctx.needs_input_grad[:3]))
+        ctx.save_for_backward(x, weight, bias, gate)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        _no_capture("linear_act")
+        x, weight, bias, gate = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dx, dw, db = _linear_bwd(dy, x, weight, gate, bias if need[2] else None, need[0], need[1])
+        return dx, dw, db, dy if need[3] else None, None
+
+
+def linear_act(x, weight, bias=None, act=ACT_NONE, residual=None, return_gate=False):
+    """y = act(x @ weight^T + bias) + residual in one launch for 16-bit tokens: x [..., K] and weight [N, K] (nn.Linear's layout) bf16 or
+    fp16, bias [N] of that type or fp32, residual [..., N], act ACT_NONE, ACT_RELU or ACT_GELU (erf). Any K >= 1 and N; widths that are
+    multiples of 8 with 16-byte aligned rows are read in place, others are copied with padded rows first. fp32 sums, one rounding.
+    Returns y [..., N] contiguous; with return_gate (y, gate): act' at the same place for linear_act_bwd (None for ACT_NONE).
+    Differentiable in x, weight, bias, residual. fp32 tokens: slot_gemm / bgemm."""
+    x, weight, residual = _linear_args(x, weight, bias, act, residual)
+    if not return_gate and torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
+        return _LinearAct.apply(x, weight, bias, residual, act)
+    with torch.no_grad():
+        y, gate = _linear_fwd(x, weight, bias, act, residual, return_gate)
+    return (y, gate) if return_gate else y
+
+
+def linear_act_bwd(dy, x, weight, gate=None, bias=None, want_dx=True, want_dw=True):
+    """Gradients (dx, dweight, dbias) of linear_act as a plain call, from the forward's gate (None: no activation). bias: the forward's
+    bias, for the type of its gradient (None: no dbias). The residual's gradient is dy itself. want_dx / want_dw = False: None there."""
+    x, weight, _ = _linear_args(x, weight, bias, ACT_NONE, None)
+    dy = _token_tensor(dy, "dy", (x.dtype,))
+    if gate is not None:
+        gate = _token_tensor(gate, "gate", (x.dtype,)).contiguous()
+    return _linear_bwd(dy, x, weight, gate, bias, want_dx, want_dw)
 
 
 class KernelTimer:
