@@ -180,34 +180,53 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void attention_fwd_kernel
     if (a.lse && h == 0) a.lse[((long long)b * a.H + head) * a.N + n] = some ? (mc + log2f(l)) * 0.69314718055994531f : -INFINITY;
 }
 
-// joins the splits of a row: o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s. One wave per row, lanes over channels.
+// joins the splits of a row: o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s. One workgroup per row: every lane of a wave holds the
+// weight of one split (splits <= 64), thread (g, c) adds splits g, g + 8, .. of channels 4 c .. 4 c + 3, the eight sums meet in LDS.
 template <typename T>
 __global__ __launch_bounds__(256) void attention_combine_kernel(AttArgs a) {
+    __shared__ float red[8][128];
+    __shared__ float wt[64];
     const long long rows = (long long)a.B * a.N * a.H;
-    const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63;
-    if (row >= rows) return;
+    const long long row = blockIdx.x;
+    const int lane = threadIdx.x & 63, g = threadIdx.x >> 5, c = (threadIdx.x & 31) * 4;
     const float* ml = a.part + (long long)a.splits * rows * a.D;
-    float m = -INFINITY;
-    for (int s = 0; s < a.splits; ++s) {
-        const float* x = ml + (s * rows + row) * 2;
-        if (x[1] > 0.f) m = fmaxf(m, x[0]);
+    float ms = -INFINITY, ls = 0.f;
+    if (lane < a.splits) {
+        const float2 x = *reinterpret_cast<const float2*>(ml + (lane * rows + row) * 2);
+        ls = x.y;
+        ms = ls > 0.f ? x.x : -INFINITY;
     }
-    float l = 0.f, o0 = 0.f, o1 = 0.f;
-    for (int s = 0; s < a.splits; ++s) {
-        const float* x = ml + (s * rows + row) * 2;
-        if (!(x[1] > 0.f)) continue;
-        const float f = exp2f(x[0] - m);
-        l += f * x[1];
-        const float* o = a.part + (s * rows + row) * a.D;
-        if (lane < a.D) o0 += f * o[lane];
-        if (lane + 64 < a.D) o1 += f * o[lane + 64];
+    float m = ms;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
+    const float f = ls > 0.f ? exp2f(ms - m) : 0.f;
+    float l = f * ls;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) l += __shfl_xor(l, o);
+    if (threadIdx.x < 64) wt[lane] = f;
+    __syncthreads();
+    f32x4 s = {0.f, 0.f, 0.f, 0.f};
+    if (c < a.D) {
+#pragma unroll 4
+        for (int k = g; k < a.splits; k += 8) {
+            const float w = wt[k];
+            if (w > 0.f) {                                         // a split without keys left its sums unwritten
+                const f32x4 o = *reinterpret_cast<const f32x4*>(a.part + (k * rows + row) * a.D + c);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) s[j] += w * o[j];
+            }
+        }
     }
+    *reinterpret_cast<f32x4*>(&red[g][c]) = s;
+    __syncthreads();
     const float inv = l > 0.f ? 1.f / l : 0.f;
-    T* dst = (T*)a.out + row * a.D;
-    if (lane < a.D) dst[lane] = (T)(o0 * inv);
-    if (lane + 64 < a.D) dst[lane + 64] = (T)(o1 * inv);
-    if (a.lse && lane == 0) {
+    if (threadIdx.x < a.D) {
+        float t = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) t += red[k][threadIdx.x];
+        ((T*)a.out)[row * a.D + threadIdx.x] = (T)(t * inv);
+    }
+    if (a.lse && threadIdx.x == 0) {
         const int h = (int)(row % a.H);
         const long long bn = row / a.H;
         const int n = (int)(bn % a.N);
@@ -251,7 +270,7 @@ static int attention_dispatch(const AttArgs& a, const AttPlan& p, hipStream_t st
     else rc = a.D <= 32 ? attention_launch<T, 32, 4, 64>(a, stream) : a.D <= 64 ? attention_launch<T, 64, 4, 64>(a, stream) : attention_launch<T, 128, 4, 64>(a, stream);
     if (rc || a.splits == 1) return rc;
     const long long rows = (long long)a.B * a.N * a.H;
-    hipLaunchKernelGGL(attention_combine_kernel<T>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL(attention_combine_kernel<T>, dim3((unsigned)rows), dim3(256), 0, stream, a);
     return (int)hipGetLastError();
 }
 

@@ -5,8 +5,8 @@
 // One product kernel serves all three: C[m, n] = sum_k X(m, k) W(n, k) with either operand stored k-contiguous ([m][k]) or k-major
 // ([k][m]): forward (contiguous, contiguous), dx (contiguous, k-major), dW (k-major, k-major). Fragments of a k-contiguous tile are 16-byte
 // LDS reads, of a k-major tile two hardware-transposed reads. Sums are fp32; bias, activation, slope and residual act on them before the
-// one rounding of y. The slope g is stored instead of the pre-activation: rounded once it is off by half a step, where the slope of a
-// rounded pre-activation would be off by the rounding times the curvature, and the backward pass needs no transcendental.
+// one rounding of y. The slope g is stored instead of the pre-activation: held as int16 in units of 2^-14 it is off by 3e-5 (a 16-bit
+// pre-activation in bf16: by up to 4e-3 times the curvature), and the backward pass needs no transcendental.
 //
 // Tile BM x BN x 64, WM x WN waves; LDS double-buffered by 16-byte LDS-DMA, one barrier per 64-deep step. The W fragment is the MFMA's row
 // operand: a lane owns one row m and four consecutive n per accumulator quad. Tiles behind each other in memory go to one XCD (its L2
@@ -35,22 +35,43 @@ template <int BYTES> __device__ __forceinline__ int lin_swz(int row) {      // r
     else return att_swz<BYTES / 2>(row);
 }
 
-// KM = false: tile of `R` rows x 64 k (row0 .. on the m / n side);  KM = true: tile of 64 k rows x R columns
+// An operand's tile of one 64-deep step. KM = false: R rows (m or n side) x 64 k;  KM = true: 64 k rows x R columns.
+// Every lane's offsets inside the tile are computed once; a step only moves the wave-uniform base. Rows (columns) behind the operand's
+// end read its last ones again: they only reach accumulators that are not stored. What lies behind K must not count: the last step of a
+// K that is no multiple of 64 takes zeros there.
 template <int R, int NW, bool KM>
-__device__ __forceinline__ void lin_stage(const char* base, long long ld, int row0, int rows, int k0, int K, char* lds, int w, int lane) {
-    constexpr int LROWS = KM ? 64 : R, BYTES = KM ? R * 2 : 128, CH = BYTES / 16, RPP = 64 / CH, PIECES = LROWS / RPP;
+struct LinTile {
+    static constexpr int LROWS = KM ? 64 : R, BYTES = KM ? R * 2 : 128, CH = BYTES / 16, RPP = 64 / CH, PIECES = LROWS / RPP, N = PIECES / NW;
+    static_assert(PIECES % NW == 0, "every wave stages the same number of pieces");
+    const char* base;                           // of the tile at k = 0
+    long long step;                             // bytes per step
+    uint32_t off[N];
+    __device__ __forceinline__ void init(const void* p, long long ld, int row0, int rows, int w, int lane) {
+        base = (const char*)p + (KM ? (long long)row0 * 2 : (long long)row0 * ld * 2);
+        step = KM ? 64 * ld * 2 : 128;
 #pragma unroll
-    for (int i = 0; i < (PIECES + NW - 1) / NW; ++i) {
-        const int j = i * NW + w;
-        if (PIECES % NW == 0 || j < PIECES) {
-            const int lr = j * RPP + lane / CH;
+        for (int i = 0; i < N; ++i) {
+            const int lr = (i * NW + w) * RPP + lane / CH;
             const int chunk = (lane % CH) ^ lin_swz<BYTES>(lr);
-            const int sr = (KM ? k0 : row0) + lr, sc = (KM ? row0 : k0) + chunk * 8;     // stored row, column
-            const bool ok = KM ? (sr < K && sc < rows) : (sr < rows && sc < K);
-            dma16(ok ? base + ((long long)sr * ld + sc) * 2 : reinterpret_cast<const char*>(g_att_zero), lds + j * 1024);
+            const int last = KM ? ((rows - 1 - row0) >> 3) : rows - 1 - row0;       // last chunk column / last row
+            off[i] = KM ? (uint32_t)(lr * ld * 2) + (chunk < last ? chunk : last) * 16 : (uint32_t)((lr < last ? lr : last) * ld * 2) + chunk * 16;
         }
     }
-}
+    __device__ __forceinline__ void stage(int s, int K, char* lds, int w, int lane) const {
+        const char* b = base + s * step;
+        if ((s + 1) * 64 <= K) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) dma16(b + off[i], lds + (i * NW + w) * 1024);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int lr = (i * NW + w) * RPP + lane / CH;
+                const int k = s * 64 + (KM ? lr : 8 * ((lane % CH) ^ lin_swz<BYTES>(lr)));
+                dma16(k < K ? b + off[i] : reinterpret_cast<const char*>(g_att_zero), lds + (i * NW + w) * 1024);
+            }
+        }
+    }
+};
 
 template <typename T, int R, bool KM>
 __device__ __forceinline__ typename AttVec<T>::v8 lin_frag(const char* lds, int row0, int ks, int lane) {
@@ -72,64 +93,67 @@ __device__ __forceinline__ typename AttVec<T>::v8 lin_frag(const char* lds, int 
     }
 }
 
+// GELU through the complementary error function's exponential form (Abramowitz and Stegun 7.1.26, |error| <= 1.5e-7):
+//   erfc(x) = exp(-x^2) t (a1 + t (a2 + t (a3 + t (a4 + t a5)))), t = 1 / (1 + p x), x = |z| / sqrt 2
+// with exp(-x^2) = exp(-z^2 / 2), the same exponential that the slope needs: one exponential and one reciprocal per value in place of
+// erff's two branches (measured at 32768 x 384 -> 1536: 154 us with erff, 96 us so).
 __device__ __forceinline__ void lin_act(int act, float z, float& y, float& g) {
     y = z;
     g = 1.f;
     if (act == kActRelu) {
-        y = fmaxf(z, 0.f);
+        y = z > 0.f ? z : z != z ? z : 0.f;
         g = z > 0.f ? 1.f : 0.f;
-        if (z != z) { y = z; g = z; }
     } else if (act == kActGelu) {
-        const float cdf = 0.5f * (1.f + erff(z * 0.70710678118654752f));
+        const float e = __builtin_amdgcn_exp2f(-0.72134752044448170f * z * z);
+        const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f * 0.70710678118654752f, fabsf(z), 1.f));
+        const float q = 0.5f * e * t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
+        const float cdf = z > 0.f ? 1.f - q : q;
         y = z * cdf;
-        g = cdf + z * 0.39894228040143268f * __builtin_amdgcn_exp2f(-0.72134752044448170f * z * z);
+        g = fmaf(z * 0.39894228040143268f, e, cdf);
+        if (!(fabsf(z) < 1e18f)) {                                 // z * z has left fp32's range: the limits, NaN stays
+            y = z > 0.f ? z : z != z ? z : 0.f;
+            g = z > 0.f ? 1.f : 0.f;
+        }
     }
 }
 
-// four consecutive columns n .. n + 3 of row m
+constexpr float kGateOne = 16384.f;               // slopes are held as int16 in units of 2^-14 (they lie in [-0.13, 1.13]): off by 3e-5 at most
+
 template <typename T>
-__device__ __forceinline__ void lin_epilogue(const LinArgs& a, int m, int n, const float* z, bool vec) {
-    typedef typename AttVec<T>::v4 v4;
+__device__ __forceinline__ float lin_bias(const LinArgs& a, int n) {
+    return !a.bias ? 0.f : a.bias_f32 ? ((const float*)a.bias)[n] : (float)((const T*)a.bias)[n];
+}
+
+// N8 consecutive columns n .. of row m and their bias (8: N % 8 == 0 and 16-byte aligned tensors; 1: any)
+template <typename T, int N8>
+__device__ __forceinline__ void lin_epilogue(const LinArgs& a, int m, int n, const float* z, const float* b) {
     const long long o = (long long)m * a.N + n;
-    float y[4], g[4];
-    if (vec) {                                                   // N % 4 == 0, 8-byte aligned tensors
-        float b[4] = {0.f, 0.f, 0.f, 0.f};
-        if (a.bias) {
-            if (a.bias_f32) {
+    float y[N8], g[N8];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) b[j] = ((const float*)a.bias)[n + j];
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) b[j] = (float)((const T*)a.bias)[n + j];
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) lin_act(a.act, z[j] + b[j], y[j], g[j]);
+    for (int j = 0; j < N8; ++j) lin_act(a.act, z[j] + b[j], y[j], g[j]);
+    if constexpr (N8 == 8) {
         if (a.residual) {
-            const v4 r = *reinterpret_cast<const v4*>((const T*)a.residual + o);
+            const typename AttVec<T>::v8 r = *reinterpret_cast<const typename AttVec<T>::v8*>((const T*)a.residual + o);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) y[j] += (float)r[j];
+            for (int j = 0; j < 8; ++j) y[j] += (float)r[j];
         }
-        v4 yo, go;
+        *reinterpret_cast<typename AttVec<T>::v8*>((T*)a.y + o) = att_pack<T>(y);
+        if (a.gate) {
+            typedef short s16x8 __attribute__((ext_vector_type(8)));
+            s16x8 q;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) { yo[j] = (T)y[j]; go[j] = (T)g[j]; }
-        *reinterpret_cast<v4*>((T*)a.y + o) = yo;
-        if (a.gate) *reinterpret_cast<v4*>((T*)a.gate + o) = go;
-        return;
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        if (n + j >= a.N) break;
-        const float b = !a.bias ? 0.f : a.bias_f32 ? ((const float*)a.bias)[n + j] : (float)((const T*)a.bias)[n + j];
-        lin_act(a.act, z[j] + b, y[j], g[j]);
-        if (a.residual) y[j] += (float)((const T*)a.residual)[o + j];
-        ((T*)a.y)[o + j] = (T)y[j];
-        if (a.gate) ((T*)a.gate)[o + j] = (T)g[j];
+            for (int j = 0; j < 8; ++j) q[j] = (short)(int)rintf(g[j] * kGateOne);
+            *reinterpret_cast<s16x8*>((short*)a.gate + o) = q;
+        }
+    } else {
+        if (a.residual) y[0] += (float)((const T*)a.residual)[o];
+        ((T*)a.y)[o] = (T)y[0];
+        if (a.gate) ((short*)a.gate)[o] = (short)(int)rintf(g[0] * kGateOne);
     }
 }
 
 __device__ __forceinline__ bool lin_vec(const LinArgs& a) {
-    return a.N % 4 == 0 && !(((uintptr_t)a.y | (uintptr_t)a.residual | (uintptr_t)a.gate) & 7);
+    return a.N % 8 == 0 && !(((uintptr_t)a.y | (uintptr_t)a.residual | (uintptr_t)a.gate) & 15);
 }
 
 template <typename T, int BM, int BN, int WM, int WN, bool XK, bool WK>
@@ -161,12 +185,14 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_kernel(LinArgs a) {
         sb = split * per;
         se = sb + per < steps ? sb + per : steps;
     }
-    const char* xb = (const char*)a.x;
-    const char* wb = (const char*)a.w;
-    auto stage = [&](int s, int buf) {
-        char* l = smem + buf * (XB + WB);
-        lin_stage<BM, NW, XK>(xb, a.ldx, m0, a.M, s * 64, a.K, l, w, lane);
-        lin_stage<BN, NW, WK>(wb, a.ldw, n0, a.N, s * 64, a.K, l + XB, w, lane);
+    LinTile<BM, NW, XK> tx;
+    LinTile<BN, NW, WK> tw;
+    tx.init(a.x, a.ldx, m0, a.M, w, lane);
+    tw.init(a.w, a.ldw, n0, a.N, w, lane);
+    auto stage = [&](int s) {
+        char* l = smem + ((s - sb) & 1) * (XB + WB);
+        tx.stage(s, a.K, l, w, lane);
+        tw.stage(s, a.K, l + XB, w, lane);
     };
     f32x16 acc[MI][NI];
 #pragma unroll
@@ -175,62 +201,130 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_kernel(LinArgs a) {
         for (int j = 0; j < NI; ++j)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-    if (sb < se) stage(sb, 0);
-    for (int s = sb; s < se; ++s) {
-        const int buf = (s - sb) & 1;
+    // Operand fragments one 16-deep slice ahead of the products. The barrier stands BEFORE the last slice's products: by then the step's
+    // tile is in registers, so the tile after next may overwrite it, the next one has had a step to arrive, and its first fragments are
+    // read under the last products.
+    v8 xf[2][MI], wf[2][NI];
+    auto fetch = [&](int s, int ks, int to) {
+        const char* lx = smem + ((s - sb) & 1) * (XB + WB);
+#pragma unroll
+        for (int i = 0; i < MI; ++i) xf[to][i] = lin_frag<T, BM, XK>(lx, (wm * MI + i) * 32, ks, lane);
+#pragma unroll
+        for (int j = 0; j < NI; ++j) wf[to][j] = lin_frag<T, BN, WK>(lx + XB, (wn * NI + j) * 32, ks, lane);
+    };
+    auto multiply = [&](int from) {
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+            for (int j = 0; j < NI; ++j) acc[i][j] = mfma16(wf[from][j], xf[from][i], acc[i][j]);
+    };
+    if (sb < se) {
+        stage(sb);
         wait_vm<0>();
         wg_barrier();
-        if (s + 1 < se) stage(s + 1, buf ^ 1);
-        const char* lx = smem + buf * (XB + WB);
-        const char* lw = lx + XB;
-#pragma unroll
-        for (int ks = 0; ks < 4; ++ks) {
-            v8 xf[MI], wf[NI];
-#pragma unroll
-            for (int i = 0; i < MI; ++i) xf[i] = lin_frag<T, BM, XK>(lx, (wm * MI + i) * 32, ks, lane);
-#pragma unroll
-            for (int j = 0; j < NI; ++j) wf[j] = lin_frag<T, BN, WK>(lw, (wn * NI + j) * 32, ks, lane);
-#pragma unroll
-            for (int i = 0; i < MI; ++i)
-#pragma unroll
-                for (int j = 0; j < NI; ++j) acc[i][j] = mfma16(wf[j], xf[i], acc[i][j]);
-        }
+        if (sb + 1 < se) stage(sb + 1);
+        fetch(sb, 0, 0);
     }
+    for (int s = sb; s < se; ++s) {
+        fetch(s, 1, 1);
+        multiply(0);
+        fetch(s, 2, 0);
+        multiply(1);
+        fetch(s, 3, 1);
+        multiply(0);
+        if (s + 1 < se) {
+            wait_vm<0>();
+            wg_barrier();
+            if (s + 2 < se) stage(s + 2);
+            fetch(s + 1, 0, 0);
+        }
+        multiply(1);
+    }
+    // Epilogue: a wave turns its 32-row blocks around through its own piece of LDS, so that 8 lanes write 128 consecutive bytes of a row
+    // (straight from the accumulators a lane would hold 4 columns of its own row: 32 rows per access, four times the cache-line visits).
+    constexpr int COLS = NI * 32, LROW = COLS * 4 + 16;
+    static_assert(NW * 32 * LROW <= 2 * (XB + WB), "the epilogue reuses the operand tiles");
+    wg_barrier();                                                  // every wave has read its last operand tile
+    char* my = smem + w * 32 * LROW;
     const bool vec = lin_vec(a);
+    constexpr int LPR = COLS / 8, RPP = 64 / LPR;                  // lanes per row, rows per pass
+    float bias[8];                                                 // a lane's columns are the same in every pass
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const int n = n0 + wn * COLS + (vec ? (lane % LPR) * 8 + j : lane + 64 * j);
+        bias[j] = n < a.N ? lin_bias<T>(a, n) : 0.f;
+    }
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
-        const int m = m0 + (wm * MI + i) * 32 + r;
-        if (m >= a.M) continue;
+        const int mb = m0 + (wm * MI + i) * 32, nb = n0 + wn * COLS;
 #pragma unroll
         for (int j = 0; j < NI; ++j)
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-                const int n = n0 + (wn * NI + j) * 32 + 8 * g + 4 * h;
-                if (n >= a.N) continue;
-                float z[4];
+                f32x4 v;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) z[e] = acc[i][j][4 * g + e];
-                if (a.splits > 1) *reinterpret_cast<f32x4*>(a.part + ((long long)split * a.M + m) * a.ldp + n) = f32x4{z[0], z[1], z[2], z[3]};
-                else lin_epilogue<T>(a, m, n, z, vec);
+                for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * g + e];
+                *reinterpret_cast<f32x4*>(my + r * LROW + (32 * j + 8 * g + 4 * h) * 4) = v;
             }
+        if (mb >= a.M || nb >= a.N) continue;
+        if (a.splits > 1 || vec) {
+#pragma unroll
+            for (int q = 0; q < 32 / RPP; ++q) {
+                const int rr = q * RPP + lane / LPR, c = (lane % LPR) * 8, m = mb + rr, n = nb + c;
+                if (m >= a.M || n >= a.N) continue;
+                float z[8];
+                *reinterpret_cast<f32x4*>(z) = *reinterpret_cast<const f32x4*>(my + rr * LROW + c * 4);
+                *reinterpret_cast<f32x4*>(z + 4) = *reinterpret_cast<const f32x4*>(my + rr * LROW + c * 4 + 16);
+                if (a.splits > 1) {                                // ldp = N rounded up to 8
+                    float* p = a.part + ((long long)split * a.M + m) * a.ldp + n;
+                    *reinterpret_cast<f32x4*>(p) = f32x4{z[0], z[1], z[2], z[3]};
+                    *reinterpret_cast<f32x4*>(p + 4) = f32x4{z[4], z[5], z[6], z[7]};
+                } else {
+                    lin_epilogue<T, 8>(a, m, n, z, bias);
+                }
+            }
+        } else {                                                   // a lane per column
+#pragma unroll
+            for (int c = 0; c < COLS / 32; c += 2) {
+                const int cc = 32 * c + lane;
+                if (cc >= COLS || nb + cc >= a.N) continue;
+#pragma unroll 4
+                for (int rr = 0; rr < 32; ++rr)
+                    if (mb + rr < a.M) {
+                        const float z = *reinterpret_cast<const float*>(my + rr * LROW + cc * 4);
+                        lin_epilogue<T, 1>(a, mb + rr, nb + cc, &z, bias + c / 2);
+                    }
+            }
+        }
     }
 }
 
-// the splits of a product added in order, then the same epilogue
+// the splits of a product added in order, then the same epilogue: 8 columns per thread
 template <typename T>
 __global__ __launch_bounds__(256) void linear_join_kernel(LinArgs a) {
     const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
-    const int cols = a.ldp >> 2;
+    const int cols = a.ldp >> 3;
     const long long m = id / cols;
-    const int n = (int)(id - m * cols) * 4;
-    if (m >= a.M || n >= a.N) return;
-    float z[4] = {0.f, 0.f, 0.f, 0.f};
+    const int n = (int)(id - m * cols) * 8;
+    if (m >= a.M) return;
+    float z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
     for (int s = 0; s < a.splits; ++s) {
-        const f32x4 v = *reinterpret_cast<const f32x4*>(a.part + ((long long)s * a.M + m) * a.ldp + n);
+        const f32x4* p = reinterpret_cast<const f32x4*>(a.part + ((long long)s * a.M + m) * a.ldp + n);
+        const f32x4 u = p[0], v = p[1];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) z[e] += v[e];
+        for (int e = 0; e < 4; ++e) { z[e] += u[e]; z[4 + e] += v[e]; }
     }
-    lin_epilogue<T>(a, (int)m, n, z, lin_vec(a));
+    float bias[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) bias[j] = n + j < a.N ? lin_bias<T>(a, n + j) : 0.f;
+    if (lin_vec(a)) {
+        lin_epilogue<T, 8>(a, (int)m, n, z, bias);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (n + j < a.N) lin_epilogue<T, 1>(a, (int)m, n + j, z + j, bias + j);
+    }
 }
 
 // [rows, cols] with row stride ld -> [rows, ldo], ldo = cols rounded up to 8, zeros behind cols. 8 columns per thread.
@@ -249,7 +343,7 @@ __global__ __launch_bounds__(256) void linear_pack_kernel(const uint16_t* src, l
 // dz = dy * gate (stored with row stride ldz, zero padded; skipped when dz is null) and the column sums of dz over a chunk of rows.
 // Workgroup: 256 columns (32 threads x 8) x 8 rows at a time over `rows_per` rows.
 template <typename T>
-__global__ __launch_bounds__(256) void linear_dz_kernel(const T* dy, long long ldy, const T* gate, T* dz, int ldz, float* sums, int M, int N, int rows_per) {
+__global__ __launch_bounds__(256) void linear_dz_kernel(const T* dy, long long ldy, const short* gate, T* dz, int ldz, float* sums, int M, int N, int rows_per) {
     typedef typename AttVec<T>::v8 v8;
     __shared__ float red[8][256];
     const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
@@ -265,9 +359,10 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(const T* dy, long long l
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[j] = (float)d[j];
             if (gate) {
-                const v8 g = *reinterpret_cast<const v8*>(gate + (long long)m * N + c0);
+                typedef short s16x8 __attribute__((ext_vector_type(8)));
+                const s16x8 g = *reinterpret_cast<const s16x8*>(gate + (long long)m * N + c0);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] *= (float)g[j];
+                for (int j = 0; j < 8; ++j) v[j] *= (float)g[j] * (1.f / kGateOne);
             }
         } else {
 #pragma unroll
@@ -275,7 +370,7 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(const T* dy, long long l
                 v[j] = 0.f;
                 if (c0 + j < N) {
                     v[j] = (float)dy[(long long)m * ldy + c0 + j];
-                    if (gate) v[j] *= (float)gate[(long long)m * N + c0 + j];
+                    if (gate) v[j] *= (float)gate[(long long)m * N + c0 + j] * (1.f / kGateOne);
                 }
             }
         }
@@ -294,12 +389,22 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(const T* dy, long long l
     if (c < N) sums[(long long)blockIdx.y * N + c] = t;
 }
 
+// db = the chunks' sums: a workgroup takes 32 columns, eight rows of threads add every eighth chunk, the eight sums meet in LDS
 template <typename T>
 __global__ __launch_bounds__(256) void linear_db_kernel(const float* sums, int chunks, int N, void* db, int db_f32) {
-    const int c = blockIdx.x * 256 + threadIdx.x;
-    if (c >= N) return;
+    __shared__ float red[8][32];
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5, c = blockIdx.x * 32 + tx;
     float t = 0.f;
-    for (int k = 0; k < chunks; ++k) t += sums[(long long)k * N + c];
+    if (c < N) {
+#pragma unroll 8
+        for (int k = ty; k < chunks; k += 8) t += sums[(long long)k * N + c];
+    }
+    red[ty][tx] = t;
+    __syncthreads();
+    if (ty || c >= N) return;
+    t = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) t += red[k][tx];
     if (db_f32) ((float*)db)[c] = t;
     else ((T*)db)[c] = (T)t;
 }
@@ -307,13 +412,17 @@ __global__ __launch_bounds__(256) void linear_db_kernel(const float* sums, int c
 static inline int round8(int x) { return (x + 7) & ~7; }
 static inline bool lin_direct(const void* p, long long ld, int cols) { return !((uintptr_t)p & 15) && !(ld & 7) && !(cols & 7); }
 
-struct LinPlan { int splits; size_t part_bytes; };
+struct LinPlan { int big, splits; size_t part_bytes; };
 
+// 256 x 256 tiles where they fill the chip (they read each operand value half as often from LDS), 128 x 128 otherwise; the k range is split
+// where even those leave half the chip idle.
 static LinPlan linear_plan(int M, int N, int K) {
     LinPlan p;
-    const long long tiles = ((M + 127LL) / 128) * ((N + 127LL) / 128), want = 2LL * svps_num_cus();
-    long long s = tiles * 2 > want ? 1 : want / tiles;
+    const int cus = svps_num_cus();
+    const long long big = ((M + 255LL) / 256) * ((N + 255LL) / 256), small = ((M + 127LL) / 128) * ((N + 127LL) / 128), want = 2LL * cus;
+    p.big = big * 4 >= cus * 3LL;
     const long long steps = (K + 63) / 64;
+    long long s = p.big || small * 2 > want ? 1 : want / small;
     if (s > steps / 2) s = steps / 2;
     if (s > 64) s = 64;
     p.splits = s < 1 ? 1 : (int)s;
@@ -321,20 +430,25 @@ static LinPlan linear_plan(int M, int N, int K) {
     return p;
 }
 
+template <typename T, int BM, int BN, int WM, int WN, bool XK, bool WK>
+static int linear_launch_tile(const LinArgs& a, hipStream_t stream) {
+    constexpr int LDS = 2 * (BM + BN) * 128;
+    static SvpsLdsAttr attr;
+    const hipError_t e = attr.ensure((const void*)linear_kernel<T, BM, BN, WM, WN, XK, WK>, LDS);
+    if (e != hipSuccess) return (int)e;
+    const unsigned grid = (unsigned)(((a.M + BM - 1LL) / BM) * ((a.N + BN - 1LL) / BN) * a.splits);
+    hipLaunchKernelGGL((linear_kernel<T, BM, BN, WM, WN, XK, WK>), dim3(grid), dim3(64 * WM * WN), LDS, stream, a);
+    return (int)hipGetLastError();
+}
+
 template <typename T, bool XK, bool WK>
 static int linear_launch(LinArgs a, const LinPlan& p, float* part, hipStream_t stream) {
-    constexpr int BM = 128, BN = 128, WM = 2, WN = 2, LDS = 2 * (BM + BN) * 128;
-    static SvpsLdsAttr attr;
-    hipError_t e = attr.ensure((const void*)linear_kernel<T, BM, BN, WM, WN, XK, WK>, LDS);
-    if (e != hipSuccess) return (int)e;
     a.splits = p.splits;
     a.part = part;
     a.ldp = round8(a.N);
-    const unsigned grid = (unsigned)(((a.M + BM - 1LL) / BM) * ((a.N + BN - 1LL) / BN) * p.splits);
-    hipLaunchKernelGGL((linear_kernel<T, BM, BN, WM, WN, XK, WK>), dim3(grid), dim3(64 * WM * WN), LDS, stream, a);
-    e = hipGetLastError();
-    if (e != hipSuccess || p.splits == 1) return (int)e;
-    const long long threads = (long long)a.M * (a.ldp >> 2);
+    const int rc = p.big ? linear_launch_tile<T, 256, 256, 2, 4, XK, WK>(a, stream) : linear_launch_tile<T, 128, 128, 2, 2, XK, WK>(a, stream);
+    if (rc || p.splits == 1) return rc;
+    const long long threads = (long long)a.M * (a.ldp >> 3);
     hipLaunchKernelGGL(linear_join_kernel<T>, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, stream, a);
     return (int)hipGetLastError();
 }
@@ -347,7 +461,8 @@ static int linear_pack(const void* src, long long ld, void* dst, int rows, int c
 
 static bool linear_shape_ok(int M, int K, int N, long long ldx, long long ldw) {
     const long long big = 1LL << 30;
-    if (M <= 0 || K <= 0 || N <= 0 || M > big || K > big || N > big || ldx < K || ldw < K) return false;
+    // 256 rows of an operand stay inside 32-bit offsets
+    if (M <= 0 || K <= 0 || N <= 0 || M > big || K > 1 << 22 || N > 1 << 22 || ldx < K || ldw < K || ldx > 1 << 22 || ldw > 1 << 22) return false;
     // workgroups, packed rows and 8-element groups of every launch fit 31 bits
     return ((M + 127LL) / 128) * ((N + 127LL) / 128) <= big / 64 && ((M + 127LL) / 128) * ((K + 127LL) / 128) <= big / 64 &&
            ((K + 127LL) / 128) * ((N + 127LL) / 128) <= big / 64;
@@ -419,7 +534,7 @@ static LinBwdPlan linear_bwd_plan(int M, int K, int N, bool own_dz, bool pack_x,
 }
 
 template <typename T>
-static int linear_bwd_t(const T* dy, long long ldy, const T* x, long long ldx, const T* w, long long ldw, const T* gate, T* dx, T* dw, void* db,
+static int linear_bwd_t(const T* dy, long long ldy, const T* x, long long ldx, const T* w, long long ldw, const short* gate, T* dx, T* dw, void* db,
                         int db_f32, char* ws, const LinBwdPlan& p, int M, int K, int N, hipStream_t s) {
     int rc;
     const T* dz = dy;
@@ -441,7 +556,7 @@ static int linear_bwd_t(const T* dy, long long ldy, const T* x, long long ldx, c
         hipError_t e = hipGetLastError();
         if (e != hipSuccess) return (int)e;
         if (sums) {
-            hipLaunchKernelGGL(linear_db_kernel<T>, dim3((N + 255) / 256), dim3(256), 0, s, sums, p.chunks, N, db, db_f32);
+            hipLaunchKernelGGL(linear_db_kernel<T>, dim3((N + 31) / 32), dim3(256), 0, s, sums, p.chunks, N, db, db_f32);
             e = hipGetLastError();
             if (e != hipSuccess) return (int)e;
         }
@@ -473,7 +588,7 @@ static int linear_bwd_t(const T* dy, long long ldy, const T* x, long long ldx, c
 extern "C" size_t svps_linear_act_bwd_workspace_bytes(int M, int K, int N, long long ldy, long long ldx, long long ldw, int unaligned, int has_gate,
                                                       int want_dx, int want_dw, int want_db) {
     using namespace svps;
-    if (!linear_shape_ok(M, K, N, ldx, ldw) || ldy < N) return 0;
+    if (!linear_shape_ok(M, K, N, ldx, ldw) || ldy < N || ldy > 1 << 22) return 0;
     const LinBwdPlan p = linear_bwd_plan(M, K, N, has_gate || unaligned || (ldy & 7) || (N & 7), unaligned || (ldx & 7) || (K & 7),
                                          unaligned || (ldw & 7) || (K & 7), want_dx, want_dw, want_db);
     return p.dz + p.x + p.w + p.sums + p.part;
@@ -485,7 +600,7 @@ extern "C" int svps_linear_act_bwd(const void* dy, long long ldy, const void* x,
     using namespace svps;
     if (!dy || (!dx && !dw && !db) || (dx && !w) || (dw && !x)) return SVPS_ERR_BAD_ARG;
     if (dtype != SVPS_DTYPE_BF16 && dtype != SVPS_DTYPE_F16) return SVPS_ERR_BAD_ARG;
-    if (!linear_shape_ok(M, K, N, x ? ldx : K, w ? ldw : K) || ldy < N) return SVPS_ERR_BAD_SHAPE;
+    if (!linear_shape_ok(M, K, N, x ? ldx : K, w ? ldw : K) || ldy < N || ldy > 1 << 22) return SVPS_ERR_BAD_SHAPE;
     if ((M + kDzRows - 1) / kDzRows > 65535) return SVPS_ERR_BAD_SHAPE;
     const LinBwdPlan p = linear_bwd_plan(M, K, N, (dx || dw) && (gate || !lin_direct(dy, ldy, N)), !lin_direct(x, ldx, K), !lin_direct(w, ldw, K),
                                          dx != nullptr, dw != nullptr, db != nullptr);
@@ -493,8 +608,8 @@ extern "C" int svps_linear_act_bwd(const void* dy, long long ldy, const void* x,
     if (need && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need)) return SVPS_ERR_WORKSPACE;
     const hipStream_t s = static_cast<hipStream_t>(stream);
     if (dtype == SVPS_DTYPE_BF16)
-        return linear_bwd_t<__bf16>((const __bf16*)dy, ldy, (const __bf16*)x, ldx, (const __bf16*)w, ldw, (const __bf16*)gate, (__bf16*)dx, (__bf16*)dw,
+        return linear_bwd_t<__bf16>((const __bf16*)dy, ldy, (const __bf16*)x, ldx, (const __bf16*)w, ldw, (const short*)gate, (__bf16*)dx, (__bf16*)dw,
                                     db, db_f32, (char*)workspace, p, M, K, N, s);
-    return linear_bwd_t<_Float16>((const _Float16*)dy, ldy, (const _Float16*)x, ldx, (const _Float16*)w, ldw, (const _Float16*)gate, (_Float16*)dx,
+    return linear_bwd_t<_Float16>((const _Float16*)dy, ldy, (const _Float16*)x, ldx, (const _Float16*)w, ldw, (const short*)gate, (_Float16*)dx,
                                   (_Float16*)dw, db, db_f32, (char*)workspace, p, M, K, N, s);
 }

@@ -20,20 +20,28 @@ class _on:
     call (kernel attributes, CU count and the launch itself are per device) and `.stream` is the current stream OF
     THAT DEVICE - not of whichever device happens to be current in the caller."""
 
+    __slots__ = ("device", "stream", "_guard")
+
     def __init__(self, *tensors):
-        devs = {t.device for t in tensors if isinstance(t, torch.Tensor)}
-        if len(devs) != 1:
-            raise ValueError(f"tensor arguments on different devices: {sorted(map(str, devs))}")
-        self.device = devs.pop()
-        if self.device.type != "cuda":
-            raise RuntimeError(f"GPU tensors only (got {self.device}); there is no CPU fallback")
+        dev = None
+        for t in tensors:
+            if isinstance(t, torch.Tensor):
+                if dev is None:
+                    dev = t.device
+                elif t.device != dev:
+                    raise ValueError(f"tensor arguments on different devices: {sorted({str(x.device) for x in tensors if isinstance(x, torch.Tensor)})}")
+        if dev is None:
+            raise ValueError("tensor arguments on different devices: []")
+        self.device = dev
+        if dev.type != "cuda":
+            raise RuntimeError(f"GPU tensors only (got {dev}); there is no CPU fallback")
         self._guard = None
 
     def __enter__(self):
         if self.device.index != torch.cuda.current_device():
             self._guard = torch.cuda.device(self.device)
             self._guard.__enter__()
-        self.stream = ctypes.c_void_p(torch.cuda.current_stream(self.device).cuda_stream)
+        self.stream = ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(self.device.index))   # current_stream() without the object: 2 us less
         return self
 
     def __exit__(self, *exc):
@@ -1143,6 +1151,12 @@ def _no_capture(what):
                            f"holds would be accumulated on that graph's stream, which ends the capture and the process; capture ops.{what}_bwd")
 
 
+@functools.lru_cache(maxsize=512)
+def _plan_bytes(fn, device, *sizes):
+    """Workspace of a launch by its sizes alone (the plan asks for the device's CU count: called with that device current)."""
+    return getattr(_lib.load(), fn)(*sizes)
+
+
 @functools.lru_cache(maxsize=64)
 def _rotary_table(split, base, ladder):
     """(int array of split, double array of frequency / (2 pi) per pair): the frequency of pair i of a section of d channels is
@@ -1187,8 +1201,8 @@ def _rotary_args(x, positions, split, base, pairing, ladder, also):
 
 def _rotary_launch(x, positions, split, base, pairing, ladder, also, inverse):
     B, N, H, D = x.shape
-    y = torch.empty((B, N, H, D), dtype=x.dtype, device=x.device)
-    y2 = None if also is None else torch.empty(also.shape, dtype=x.dtype, device=x.device)
+    y = x.new_empty((B, N, H, D))
+    y2 = None if also is None else also.new_empty(also.shape)
     if also is not None and also.shape[2] == 0:
         also = None
     if H == 0 and also is not None:                              # the launch needs a first tensor with heads
@@ -1299,7 +1313,7 @@ def _att_fwd(q, k, v, q_lens, k_lens, frame, window, scale, want_lse):
     B, N, H, D = q.shape
     M, Hk = k.shape[1], k.shape[2]
     empty = B == 0 or N == 0 or M == 0
-    out = (torch.zeros if empty else torch.empty)((B, N, H, D), dtype=q.dtype, device=q.device)
+    out = q.new_zeros((B, N, H, D)) if empty else q.new_empty((B, N, H, D))
     lse = torch.empty((B, H, N), dtype=torch.float32, device=q.device) if want_lse else None
     if empty:
         if lse is not None:
@@ -1307,7 +1321,7 @@ def _att_fwd(q, k, v, q_lens, k_lens, frame, window, scale, want_lse):
         return out, lse
     lib = _lib.load()
     with _on(q, k, v, out, lse, q_lens, k_lens) as ctx:
-        nbytes = lib.svps_attention_workspace_bytes(B, N, M, H, Hk, D)
+        nbytes = _plan_bytes("svps_attention_workspace_bytes", ctx.device.index, B, N, M, H, Hk, D)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
         rc = lib.svps_attention_fwd(q.data_ptr(), _att_strides(q), k.data_ptr(), _att_strides(k), v.data_ptr(), _att_strides(v),
                                     out.data_ptr(), _ptr(lse), _ptr(q_lens), _ptr(k_lens), _ptr(ws), nbytes, B, N, M, H, Hk, D,
@@ -1333,7 +1347,7 @@ def _att_bwd(dout, q, k, v, out, lse, q_lens, k_lens, frame, window, scale):
         return dq, dk, dv
     lib = _lib.load()
     with _on(dout, q, k, v, out, lse, q_lens, k_lens) as ctx:
-        nbytes = lib.svps_attention_bwd_workspace_bytes(B, N, M, H, Hk, D)
+        nbytes = _plan_bytes("svps_attention_bwd_workspace_bytes", ctx.device.index, B, N, M, H, Hk, D)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
         rc = lib.svps_attention_bwd(dout.data_ptr(), _att_strides(dout), q.data_ptr(), _att_strides(q), k.data_ptr(), _att_strides(k),
                                     v.data_ptr(), _att_strides(v), out.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
@@ -1390,7 +1404,7 @@ def _rows16(t, name, dtype, cols):
     """[..., cols] -> 2-D rows with contiguous columns and a row stride >= cols (a view where that is possible)."""
     t = _token_tensor(t, name, (dtype,))
     t = t.reshape(-1, cols)
-    if (cols > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < cols):
+    if (cols > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and not cols <= t.stride(0) <= 1 << 22):
         t = t.contiguous()
     return t
 
@@ -1406,6 +1420,8 @@ def _linear_args(x, weight, bias, act, residual):
     N, K = weight.shape
     if x.shape[-1] != K or K == 0:
         raise ValueError(f"linear_act: x {tuple(x.shape)} does not match weight {tuple(weight.shape)}")
+    if max(K, N) > 1 << 22:
+        raise ValueError("linear_act: at most 2^22 channels on either side")
     weight = _rows16(weight, "weight", x.dtype, K)
     if act not in (ACT_NONE, ACT_RELU, ACT_GELU):
         raise ValueError("linear_act: act must be ACT_NONE, ACT_RELU or ACT_GELU")
@@ -1426,8 +1442,8 @@ def _linear_args(x, weight, bias, act, residual):
 def _linear_fwd(x, weight, bias, act, residual, want_gate):
     N, K = weight.shape
     shape = x.shape[:-1] + (N,)
-    y = torch.empty(shape, dtype=x.dtype, device=x.device)
-    gate = torch.empty(shape, dtype=x.dtype, device=x.device) if want_gate and act != ACT_NONE else None
+    y = x.new_empty(shape)
+    gate = x.new_empty(shape, dtype=torch.int16) if want_gate and act != ACT_NONE else None
     x2 = _rows16(x, "x", x.dtype, K) if x.numel() else x
     M = y.numel() // N if N else 0
     if M == 0:
@@ -1435,7 +1451,7 @@ def _linear_fwd(x, weight, bias, act, residual, want_gate):
     lib = _lib.load()
     with _on(x, weight, bias, residual, y) as ctx:
         ldx, ldw = _ld(x2), _ld(weight)
-        nbytes = lib.svps_linear_act_workspace_bytes(M, K, N, ldx, ldw, (x2.data_ptr() | weight.data_ptr()) & 15)
+        nbytes = _plan_bytes("svps_linear_act_workspace_bytes", ctx.device.index, M, K, N, ldx, ldw, (x2.data_ptr() | weight.data_ptr()) & 15)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
         rc = lib.svps_linear_act_fwd(x2.data_ptr(), ldx, weight.data_ptr(), ldw, _ptr(bias), int(bias is not None and bias.dtype == torch.float32),
                                      _ptr(residual), int(act), y.data_ptr(), _ptr(gate), _ptr(ws), nbytes, M, K, N, _DTYPE_CODE[x.dtype], ctx.stream)
@@ -1459,8 +1475,9 @@ def _linear_bwd(dy, x, weight, gate, bias, want_dx, want_dw):
     lib = _lib.load()
     with _on(dy, x, weight, gate, bias) as ctx:
         ldy, ldx, ldw = _ld(dy2), _ld(x2), _ld(weight)
-        nbytes = lib.svps_linear_act_bwd_workspace_bytes(M, K, N, ldy, ldx, ldw, (x2.data_ptr() | weight.data_ptr() | dy2.data_ptr()) & 15,
-                                                         int(gate is not None), int(want_dx), int(want_dw), int(db is not None))
+        nbytes = _plan_bytes("svps_linear_act_bwd_workspace_bytes", ctx.device.index, M, K, N, ldy, ldx, ldw,
+                             (x2.data_ptr() | weight.data_ptr() | dy2.data_ptr()) & 15, int(gate is not None), int(want_dx), int(want_dw),
+                             int(db is not None))
         ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
         rc = lib.svps_linear_act_bwd(dy2.data_ptr(), ldy, x2.data_ptr(), ldx, weight.data_ptr(), ldw, _ptr(gate), _ptr(dx), _ptr(dw), _ptr(db),
                                      int(db is not None and db.dtype == torch.float32), _ptr(ws), nbytes, M, K, N, _DTYPE_CODE[x.dtype], ctx.stream)
@@ -1489,7 +1506,8 @@ def linear_act(x, weight, bias=None, act=ACT_NONE, residual=None, return_gate=Fa
     """y = act(x @ weight^T + bias) + residual in one launch for 16-bit tokens: x [..., K] and weight [N, K] (nn.Linear's layout) bf16 or
     fp16, bias [N] of that type or fp32, residual [..., N], act ACT_NONE, ACT_RELU or ACT_GELU (erf). Any K >= 1 and N; widths that are
     multiples of 8 with 16-byte aligned rows are read in place, others are copied with padded rows first. fp32 sums, one rounding.
-    Returns y [..., N] contiguous; with return_gate (y, gate): act' at the same place for linear_act_bwd (None for ACT_NONE).
+    Returns y [..., N] contiguous; with return_gate (y, gate) without an autograd graph: act' at the same place for
+    linear_act_bwd, int16 in units of 2^-14 (None for ACT_NONE).
     Differentiable in x, weight, bias, residual. fp32 tokens: slot_gemm / bgemm."""
     x, weight, residual = _linear_args(x, weight, bias, act, residual)
     if not return_gate and torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
@@ -1505,7 +1523,7 @@ def linear_act_bwd(dy, x, weight, gate=None, bias=None, want_dx=True, want_dw=Tr
     x, weight, _ = _linear_args(x, weight, bias, ACT_NONE, None)
     dy = _token_tensor(dy, "dy", (x.dtype,))
     if gate is not None:
-        gate = _token_tensor(gate, "gate", (x.dtype,)).contiguous()
+        gate = _token_tensor(gate, "gate", (torch.int16,)).contiguous()
     return _linear_bwd(dy, x, weight, gate, bias, want_dx, want_dw)
 
 

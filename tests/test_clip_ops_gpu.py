@@ -7,8 +7,8 @@ Tolerances, derived before the first run; u = eps / 2 of the type (half a step o
               dv:  u |dv| + (u + 2e-4) sum_i p |dO|, fp16 + 2^-25 sum |dO|
               dq, dk: every ds rounded once and p relative 2e-4, delta from the rounded output: e_i = sum_d |dO| (2 u + 2e-4) (p |v|)_d;
               u |dq| + scale sum_j ((u + 4e-4) |ds| + p (e_i + 1e-5 sum |dO v|)) |k|, fp16 + 2^-25 scale sum |k|; dk the same over i
-  dense       z: 2 K 2^-24 sum |x w|; y: u |y| + 1.2 z-error + 2^-20 (|z| + |r|); gate rounded once, dz once:
-              dx: u |dx| + (2 u + 2^-20) sum |dz w| + sum |dy| z-error |w|, fp16 + 2^-25 sum |w|; dW alike; db: one rounding of the gate
+  dense       z: 2 K 2^-24 sum |x w|; y: u |y| + 1.2 z-error + 2^-20 (|z| + |r|); gate in steps of 2^-14, dz rounded once:
+              dx: u |dx| + u sum |dz w| + sum |dy| (2^-15 + 2^-20 + z-error) |w|, fp16 + 2^-25 sum |w|; dW alike; db: the gate's step
 """
 import math
 
@@ -350,19 +350,21 @@ def test_linear_act_forward_and_gradients(cuda, dt, case):
         assert gate is None
     else:
         ezg = ez * (act == ops.ACT_GELU) + (2.0 ** -20 if act == ops.ACT_GELU else 0.0)
-        _close(gate, slope, u * slope.abs() + ezg + sb, "gate")
+        assert gate.dtype == torch.int16
+        _close(gate.double() / 2 ** 14, slope, 2.0 ** -15 + ezg, "gate")
     dx, dw, db = ops.linear_act_bwd(dy, x, w, gate=gate, bias=b)
     dyd = dy.double()
     dz = dyd * slope
-    # one rounding of the gate, one of dz (none of either without an activation: dz is dy)
-    edz = (dz.abs() * (2 * u + u * u) + dyd.abs() * ((ez if act == ops.ACT_GELU else 0) + 2.0 ** -20 + sb) + sb) if act != ops.ACT_NONE else torch.zeros_like(dz)
+    # the gate's step and one rounding of dz (none of either without an activation: dz is dy)
+    eg = dyd.abs() * ((ez if act == ops.ACT_GELU else 0) + 2.0 ** -20 + 2.0 ** -15)
+    edz = (dz.abs() + eg) * u + eg + sb if act != ops.ACT_NONE else torch.zeros_like(dz)
     rx, rw = dz @ wd, dz.t() @ xd
     _close(dx, rx, u * rx.abs() + edz @ wd.abs() + 2 * N * 2.0 ** -24 * (dz.abs() @ wd.abs()) + sb, "dx")
     _close(dw, rw, u * rw.abs() + edz.t() @ xd.abs() + 2 * M * 2.0 ** -24 * (dz.t().abs() @ xd.abs()) + sb, "dw")
     if has_b:
         rb = dz.sum(0)
         assert db.dtype == b.dtype
-        _close(db, rb, _u(b.dtype) * rb.abs() + edz.sum(0) + 2 * M * 2.0 ** -24 * dz.abs().sum(0) + sb, "db")
+        _close(db, rb, _u(b.dtype) * rb.abs() + (eg.sum(0) if act != ops.ACT_NONE else 0) + 2 * M * 2.0 ** -24 * dz.abs().sum(0) + sb, "db")
     else:
         assert db is None
     again = ops.linear_act_bwd(dy, x, w, gate=gate, bias=b)
