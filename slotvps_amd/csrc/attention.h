@@ -84,44 +84,95 @@ template <int DP> __device__ __forceinline__ int att_swz(int row) {
 
 static __device__ __attribute__((aligned(16))) uint32_t g_att_zero[4];       // never written: the source of padded rows and channels
 
+// LDS-DMA with a wave-uniform base (64-bit, in scalar registers) and a 32-bit lane offset below 2 GiB: no vector arithmetic, one register
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t dma_base(const char* base) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, 0x7fffffff, 0x00027000);
+}
+__device__ __forceinline__ void dma_off(__amdgpu_buffer_rsrc_t base, uint32_t lane_off, char* lds_base) {          // 16 bytes per lane
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(base, (SVPS_LDS void*)lds_base, 16, lane_off, 0, 0, 0);
+}
+__device__ __forceinline__ void dma_off4(__amdgpu_buffer_rsrc_t base, uint32_t lane_off, char* lds_base) {         // 4 bytes per lane
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(base, (SVPS_LDS void*)lds_base, 4, lane_off, 0, 0, 0);
+}
+
 template <typename T> struct AttVec;
 template <> struct AttVec<__bf16> { typedef bf16x8 v8; typedef bf16x4 v4; };
 template <> struct AttVec<_Float16> { typedef f16x8 v8; typedef f16x4 v4; };
 
-// ROWS rows of a [.., D] matrix into an LDS tile by 16-byte LDS-DMA; `addr(row)` gives a row's global address or null (zeros)
-template <int DP, int ROWS, int NW, typename F>
-__device__ __forceinline__ void att_stage(char* lds, int w, int lane, int D, F addr) {
-    constexpr int CH = DP / 8, RPP = 64 / CH, PIECES = ROWS / RPP;
+// ROWS packed rows of a [tokens, heads, D] operand into an LDS tile by 16-byte LDS-DMA. Packed row rr is token rr / G, head rr % G of the
+// group (keys and values: G = 1). For whole tiles of DP channels a lane's offsets are the same in every tile and only the wave-uniform
+// base moves (no address arithmetic in the loop); rows behind the last valid one and padded channels take zeros on a slower path - what
+// stands behind a length must not reach a product, 0 * NaN included.
+template <int DP, int ROWS, int NW>
+struct AttTile {
+    static constexpr int CH = DP / 8, RPP = 64 / CH, PIECES = ROWS / RPP, N = PIECES / NW, LEAP = RPP * NW;
+    static constexpr int NOFF = LEAP % 16 == 0 ? 1 : N;     // pieces 16 k rows apart have the same swizzle: one offset, the rest is uniform
+    static_assert(PIECES % NW == 0, "every wave stages the same number of pieces");
+    const char* base;
+    long long sn, sh, step, leap;               // bytes: token, head, tile, piece
+    uint32_t off[NOFF];
+    bool quick;
+    __device__ __forceinline__ void init(const void* p, long long token, long long head, const AttArgs& a, int G, int w, int lane) {
+        base = (const char*)p;
+        sn = token * 2;
+        sh = head * 2;
+        step = sn * (ROWS / G);
+        leap = NOFF == 1 ? sn * (LEAP / G) : 0;
+        quick = a.D == DP && ROWS % G == 0 && (NOFF > 1 || LEAP % G == 0) && (unsigned long long)(step + sh * G) < 0x80000000ULL;
 #pragma unroll
-    for (int i = 0; i < (PIECES + NW - 1) / NW; ++i) {
-        const int j = i * NW + w;
-        if (PIECES % NW == 0 || j < PIECES) {
-            const int row = j * RPP + lane / CH;
-            const int chunk = (lane % CH) ^ att_swz<DP>(row);
-            const char* p = addr(row);
-            const char* src = (p && chunk * 8 < D) ? p + chunk * 16 : reinterpret_cast<const char*>(g_att_zero);
-            dma16(src, lds + j * 1024);
+        for (int i = 0; i < NOFF; ++i) {
+            const int row = (i * NW + w) * RPP + lane / CH, n = G == 1 ? row : row / G;
+            off[i] = (uint32_t)(n * sn + (row - n * G) * sh) + (((lane % CH) ^ att_swz<DP>(row)) << 4);
         }
     }
+    // tile number `tile` of `rows` valid packed rows
+    __device__ __forceinline__ void stage(const AttArgs& a, int G, int tile, int rows, char* lds, int w, int lane) const {
+        if (quick && (tile + 1) * ROWS <= rows) {
+            const char* b = base + tile * step;
+#pragma unroll
+            for (int i = 0; i < N; ++i) dma_off(dma_base(b + i * leap), off[NOFF == 1 ? 0 : i], lds + (i * NW + w) * 1024);
+            return;
+        }
+#pragma unroll 1
+        for (int i = 0; i < N; ++i) {
+            const int lr = (i * NW + w) * RPP + lane / CH, row = tile * ROWS + lr;
+            const int chunk = (lane % CH) ^ att_swz<DP>(lr);
+            const int n = G == 1 ? row : att_div_g(a, row);
+            const char* p = base + n * sn + (row - n * G) * sh + chunk * 16;
+            dma16(row < rows && chunk * 8 < a.D ? p : reinterpret_cast<const char*>(g_att_zero), lds + (i * NW + w) * 1024);
+        }
+    }
+};
+
+// A lane's place in a tile, for both kinds of fragment reads. The swizzle only flips bits 4 .. 7 of an address and repeats every 16 rows,
+// so the slice (ks) and the channel block (db) are flips of the same bits: one register per kind, one exclusive-or per read.
+template <int DP>
+struct AttLane {
+    int row, col;
+    __device__ __forceinline__ AttLane(int lane) {
+        const int r = lane & 31, h = lane >> 5;
+        row = r * (DP * 2) + ((h ^ att_swz<DP>(r)) << 4);
+        const int g = lane >> 4, i = lane & 15, q = i >> 2, p = i & 3, ra = 4 * (g >> 1) + q;
+        col = ra * (DP * 2) + (((2 * (g & 1) + (p >> 1)) ^ att_swz<DP>(ra)) << 4) + 8 * (p & 1);
+    }
+    // in front of a loop body: keeps the flipped addresses of all slices from being computed outside and held there (16 registers)
+    __device__ __forceinline__ void pin() { asm volatile("" : "+v"(row), "+v"(col)); }
+};
+
+// row fragment: lane (r, h) gets channels 16 ks + 8 h .. + 8 of tile row row0 + r (row0 % 16 == 0)
+template <typename T, int DP>
+__device__ __forceinline__ typename AttVec<T>::v8 att_row_frag(const char* lds, const AttLane<DP>& at, int row0, int ks) {
+    return *reinterpret_cast<const typename AttVec<T>::v8*>(lds + row0 * (DP * 2) + (at.row ^ (ks << 5)));
 }
 
-// row fragment: lane (r, h) gets channels 16 ks + 8 h .. + 8 of tile row `row`
+// transposed fragment: lane (r, h) gets channel 32 db + r of tile rows row0 + 4h + {0..3} and row0 + 8 + 4h + {0..3} (row0 % 16 == 0;
+// eight rows further the swizzle flips bit 5)
 template <typename T, int DP>
-__device__ __forceinline__ typename AttVec<T>::v8 att_row_frag(const char* lds, int row, int ks, int h) {
-    return *reinterpret_cast<const typename AttVec<T>::v8*>(lds + row * (DP * 2) + (((2 * ks + h) ^ att_swz<DP>(row)) << 4));
-}
-
-// transposed fragment: lane (r, h) gets channel 32 db + r of tile rows row0 + 4h + {0..3} and row0 + 8 + 4h + {0..3}
-template <typename T, int DP>
-__device__ __forceinline__ typename AttVec<T>::v8 att_col_frag(const char* lds, int row0, int db, int lane) {
+__device__ __forceinline__ typename AttVec<T>::v8 att_col_frag(const char* lds, const AttLane<DP>& at, int row0, int db) {
     typedef typename AttVec<T>::v4 v4;
-    const int g = lane >> 4, i = lane & 15, q = i >> 2, p = i & 3;
-    const int ra = row0 + 4 * (g >> 1) + q, rb = ra + 8;
-    const int chunk = 4 * db + 2 * (g & 1) + (p >> 1);
-    const char* pa = lds + ra * (DP * 2) + ((chunk ^ att_swz<DP>(ra)) << 4) + 8 * (p & 1);
-    const char* pb = lds + rb * (DP * 2) + ((chunk ^ att_swz<DP>(rb)) << 4) + 8 * (p & 1);
-    const v4 lo = ds_tr16((SVPS_LDS v4*)pa);
-    const v4 hi = ds_tr16((SVPS_LDS v4*)pb);
+    const char* base = lds + row0 * (DP * 2);
+    const v4 lo = ds_tr16((SVPS_LDS v4*)(base + (at.col ^ (db << 6))));
+    const v4 hi = ds_tr16((SVPS_LDS v4*)(base + 8 * (DP * 2) + (at.col ^ 32 ^ (db << 6))));
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
@@ -133,6 +184,9 @@ __device__ __forceinline__ typename AttVec<T>::v8 att_pack(const float* x) {
     for (int j = 0; j < 8; ++j) r[j] = (T)x[j];
     return r;
 }
+
+// the reference point of a row that has seen no key: far below any score, finite, so that 2^(s - it) of a masked score is 0 and not NaN
+constexpr float kAttFloor = -3.0e38f;
 
 // a lane's 16 accumulator values of one 32-channel block (channels (i & 3) + 8 (i >> 2) + 4 h) of one row, times f, as 16-bit channels
 template <typename T>

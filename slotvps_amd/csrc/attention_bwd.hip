@@ -111,13 +111,13 @@ __global__ __launch_bounds__(256, 2) void att_dq_kernel(AttArgs a) {
             df[ks] = __builtin_bit_cast(v8, y);
         }
     }
-    const char* kbase = (const char*)((const T*)a.k + b * a.skb + hk * a.skh);
-    const char* vbase = (const char*)((const T*)a.v + b * a.svb + hk * a.svh);
-    auto stage = [&](int tile, int buf) {
+    AttTile<DP, KT, NW> tk, tv;
+    tk.init((const T*)a.k + b * a.skb + hk * a.skh, a.skn, 0, a, 1, w, lane);
+    tv.init((const T*)a.v + b * a.svb + hk * a.svh, a.svn, 0, a, 1, w, lane);
+    auto stage = [&](int tile, int buf) __attribute__((always_inline)) {
         char* lk = smem + buf * 2 * TILE;
-        const int k0 = tile * KT;
-        att_stage<DP, KT, NW>(lk, w, lane, a.D, [&](int rr) { const int key = k0 + rr; return key < klen ? kbase + (long long)key * a.skn * 2 : nullptr; });
-        att_stage<DP, KT, NW>(lk + TILE, w, lane, a.D, [&](int rr) { const int key = k0 + rr; return key < klen ? vbase + (long long)key * a.svn * 2 : nullptr; });
+        tk.stage(a, 1, tile, klen, lk, w, lane);
+        tv.stage(a, 1, tile, klen, lk + TILE, w, lane);
     };
     f32x16 acc[DB];
 #pragma unroll
@@ -125,6 +125,7 @@ __global__ __launch_bounds__(256, 2) void att_dq_kernel(AttArgs a) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[db][i] = 0.f;
     const float c = a.scale * kLog2e;
+    AttLane<DP> at(lane);
     if (tb < te) stage(tb, 0);
     for (int tile = tb; tile < te; ++tile) {
         const int buf = (tile - tb) & 1;
@@ -135,6 +136,7 @@ __global__ __launch_bounds__(256, 2) void att_dq_kernel(AttArgs a) {
         if (!wave_on || k0 >= hi_max || k0 + KT <= lo_min) continue;
         const char* lk = smem + buf * 2 * TILE;
         const char* lv = lk + TILE;
+        at.pin();
         const bool whole = k0 >= lo_max && k0 + KT <= hi_min;
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
@@ -143,8 +145,8 @@ __global__ __launch_bounds__(256, 2) void att_dq_kernel(AttArgs a) {
             for (int i = 0; i < 16; ++i) { s[i] = 0.f; dp[i] = 0.f; }
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
-                s = mfma16(att_row_frag<T, DP>(lk, 32 * kb + r, ks, h), qf[ks], s);
-                dp = mfma16(att_row_frag<T, DP>(lv, 32 * kb + r, ks, h), df[ks], dp);
+                s = mfma16(att_row_frag<T, DP>(lk, at, 32 * kb, ks), qf[ks], s);
+                dp = mfma16(att_row_frag<T, DP>(lv, at, 32 * kb, ks), df[ks], dp);
             }
             float ds[16];
 #pragma unroll
@@ -153,6 +155,7 @@ __global__ __launch_bounds__(256, 2) void att_dq_kernel(AttArgs a) {
                 ds[i] = p * (dp[i] - delta);
             }
             if (!whole) {
+                asm volatile("");                                  // a branch, not 16 selects in every tile
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     const int key = k0 + 32 * kb + acc_row(i, h);
@@ -163,7 +166,7 @@ __global__ __launch_bounds__(256, 2) void att_dq_kernel(AttArgs a) {
             for (int u = 0; u < 2; ++u) {
                 const v8 pf = att_pack<T>(ds + 8 * u);
 #pragma unroll
-                for (int db = 0; db < DB; ++db) acc[db] = mfma16(att_col_frag<T, DP>(lk, 32 * kb + 16 * u, db, lane), pf, acc[db]);
+                for (int db = 0; db < DB; ++db) acc[db] = mfma16(att_col_frag<T, DP>(lk, at, 32 * kb + 16 * u, db), pf, acc[db]);
             }
         }
     }
@@ -179,25 +182,30 @@ __global__ __launch_bounds__(256, 2) void att_dq_kernel(AttArgs a) {
     for (int db = 0; db < DB; ++db) att_store_block<T>(o, 32 * db, h, a.D, acc[db], a.scale);
 }
 
-template <typename T, int DP, int QT>
-__global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void att_dkdv_kernel(AttArgs a) {
+// dK, dV of 128 keys: KG blocks of 32 keys per wave, RG groups of waves that take turns at the row blocks (4 / RG groups of keys).
+//   DP <= 64: KG = 1, RG = 1, two waves per SIMD hide each other's waits (the exponentials bound it)
+//   DP = 128: KG = 2, RG = 2: a fragment read from LDS serves two products (with one, LDS reads and products would take the same time and
+//   neither would run at its rate); 128 + 256 registers of operands and sums leave one wave per SIMD, the two row groups add up at the end
+// (lse, delta) of a tile's rows come by LDS-DMA with the rows.
+template <typename T, int DP, int KG, int RG>
+__global__ __launch_bounds__(256, 2) void att_dkdv_kernel(AttArgs a) {
     typedef typename AttVec<T>::v8 v8;
-    constexpr int KS = DP / 16, DB = DP / 32, QB = QT / 32, TILE = QT * DP * 2, NW = 4;
+    constexpr int KS = DP / 16, DB = DP / 32, QT = 64, TILE = QT * DP * 2, NW = 4, BUF = 2 * TILE + 512, GROUPS = NW / RG;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int kg = w % GROUPS, rg = w / GROUPS;
     const int pairs = a.B * a.Hk;
     const int id = blockIdx.x, pair = id % pairs, rest = id / pairs;
-    const int t = rest % a.tiles, split = rest / a.tiles;          // early keys are seen by the most rows: longest first
+    const int t = rest / a.splits, split = rest - t * a.splits;    // early keys are seen by the most rows: longest first
     const int b = pair / a.Hk, hk = pair - b * a.Hk;
     const int qlen = att_qlen(a, b), klen = att_klen(a, b);
-    const int wk0 = t * 32 * NW, k0 = wk0 + 32 * w, key = k0 + r;
-    const bool have = key < klen;
+    const int wk0 = t * 128, k0 = wk0 + 32 * KG * kg;
 
     // tokens that see a key of [wk0, wk1): their frame is not before the first key's, and not `window` or more behind the last key's
     int n0 = 0, n1 = wk0 < klen ? qlen : 0;
     if (a.frame > 0 && n1 > 0) {
-        const int wk1 = wk0 + 32 * NW < klen ? wk0 + 32 * NW : klen;
+        const int wk1 = wk0 + 128 < klen ? wk0 + 128 : klen;
         const long long off = (long long)klen - qlen;
         const long long first = (long long)(wk0 / a.frame) * a.frame - off;
         if (first > 0) n0 = first < qlen ? (int)first : qlen;
@@ -217,119 +225,202 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void att_dkdv_kernel(AttArg
         te = tb + per < te ? tb + per : te;
     }
 
-    v8 kf[KS], vf[KS];
-    {
+    v8 kf[KG][KS], vf[KG][KS];
+#pragma unroll
+    for (int g = 0; g < KG; ++g) {
+        const int key = k0 + 32 * g + r;
         const T* kp = (const T*)a.k + b * a.skb + hk * a.skh + (long long)key * a.skn;
         const T* vp = (const T*)a.v + b * a.svb + hk * a.svh + (long long)key * a.svn;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
             const int d = 16 * ks + 8 * h;
             u32x4 x = {0, 0, 0, 0}, y = {0, 0, 0, 0};
-            if (have && d < a.D) {
+            if (key < klen && d < a.D) {
                 x = *reinterpret_cast<const u32x4*>(kp + d);
                 y = *reinterpret_cast<const u32x4*>(vp + d);
             }
-            kf[ks] = __builtin_bit_cast(v8, x);
-            vf[ks] = __builtin_bit_cast(v8, y);
+            kf[g][ks] = __builtin_bit_cast(v8, x);
+            vf[g][ks] = __builtin_bit_cast(v8, y);
         }
     }
-    const char* qbase = (const char*)((const T*)a.q + b * a.sqb + hk * a.G * a.sqh);
-    const char* dbase = (const char*)((const T*)a.dout + b * a.sdb + hk * a.G * a.sdh);
-    auto stage = [&](int tile, int buf) {
-        char* lq = smem + buf * 2 * TILE;
-        auto at = [&](const char* base, long long sn, long long sh, int rr) -> const char* {
-            const int row = tile * QT + rr, n = att_div_g(a, row);
-            return n < qlen ? base + ((long long)n * sn + (long long)(row - n * a.G) * sh) * 2 : nullptr;
-        };
-        att_stage<DP, QT, NW>(lq, w, lane, a.D, [&](int rr) { return at(qbase, a.sqn, a.sqh, rr); });
-        att_stage<DP, QT, NW>(lq + TILE, w, lane, a.D, [&](int rr) { return at(dbase, a.sdn, a.sdh, rr); });
-    };
-    f32x16 dk[DB], dv[DB];
-#pragma unroll
-    for (int db = 0; db < DB; ++db)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) { dk[db][i] = 0.f; dv[db][i] = 0.f; }
-    const float c = a.scale * kLog2e;
     const long long pbase = (long long)pair * a.rows_pad;
+    AttTile<DP, QT, NW> tq, td;
+    tq.init((const T*)a.q + b * a.sqb + hk * a.G * a.sqh, a.sqn, a.sqh, a, a.G, w, lane);
+    td.init((const T*)a.dout + b * a.sdb + hk * a.G * a.sdh, a.sdn, a.sdh, a, a.G, w, lane);
+    auto stage = [&](int tile, int buf) __attribute__((always_inline)) {
+        char* lq = smem + buf * BUF;
+        tq.stage(a, a.G, tile, qlen * a.G, lq, w, lane);
+        td.stage(a, a.G, tile, qlen * a.G, lq + TILE, w, lane);
+        if (w < 2) {                                               // 64 rows of lse2 (wave 0) and delta (wave 1); rows_pad is a multiple of 128
+            const float* src = (w ? a.stat_delta : a.stat_lse2) + pbase + tile * QT;
+            dma_off4(dma_base((const char*)src), lane * 4, lq + 2 * TILE + 256 * w);
+        }
+    };
+    f32x16 dk[KG][DB], dv[KG][DB];
+#pragma unroll
+    for (int g = 0; g < KG; ++g)
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) { dk[g][db][i] = 0.f; dv[g][db][i] = 0.f; }
+    const float c = a.scale * kLog2e;
+    AttLane<DP> at(lane);
     if (tb < te) stage(tb, 0);
     for (int tile = tb; tile < te; ++tile) {
         const int buf = (tile - tb) & 1;
         wait_vm<0>();
         wg_barrier();
         if (tile + 1 < te) stage(tile + 1, buf ^ 1);
-        const char* lq = smem + buf * 2 * TILE;
+        const char* lq = smem + buf * BUF;
         const char* ld = lq + TILE;
-#pragma unroll
-        for (int qb = 0; qb < QB; ++qb) {
+#pragma unroll 1
+        for (int qb = rg; qb < QT / 32; qb += RG) {
             const int row0 = tile * QT + 32 * qb;
-            const long long pr = pbase + row0;                     // rows_pad is a multiple of 128: in range, padding holds lse2 = inf
-            // interval bounds never fall: first and last row of the block decide whether comparisons are needed, or anything at all
-            const int nlast = att_div_g(a, row0 + 31);
-            const bool tail = nlast >= qlen;
-            const int lo_last = a.stat_lo[pr + 31], hi_first = a.stat_hi[pr], lo_first = a.stat_lo[pr];
-            const bool whole = !tail && k0 >= lo_last && k0 + 32 <= hi_first;
-            if (k0 >= klen || k0 + 32 <= lo_first) continue;
-            f32x16 s, dp;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) { s[i] = 0.f; dp[i] = 0.f; }
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                s = mfma16(att_row_frag<T, DP>(lq, 32 * qb + r, ks, h), kf[ks], s);
-                dp = mfma16(att_row_frag<T, DP>(ld, 32 * qb + r, ks, h), vf[ks], dp);
+            // interval bounds never fall along the rows: those of the block's first and last token decide whether comparisons are needed, or anything
+            const int nf = att_div_g(a, row0), nl = att_div_g(a, row0 + 31);
+            if (k0 >= klen || nf >= qlen) continue;
+            bool whole = nl < qlen && k0 + 32 * KG <= klen;
+            if (a.frame > 0) {
+                int lo_f, hi_f, lo_l, hi_l;
+                att_range(a, nf, qlen, klen, lo_f, hi_f);
+                att_range(a, nl < qlen ? nl : qlen - 1, qlen, klen, lo_l, hi_l);
+                if (k0 + 32 * KG <= lo_f || k0 >= hi_l) continue;
+                whole = whole && k0 >= lo_l && k0 + 32 * KG <= hi_f;
             }
-            float p[16], ds[16];
+            at.pin();
+            const float* st = reinterpret_cast<const float*>(lq + 2 * TILE) + 32 * qb + 4 * h;
+            v8 pf[KG][2], sf[KG][2];
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const f32x4 ls = *reinterpret_cast<const f32x4*>(a.stat_lse2 + pr + 8 * g + 4 * h);
-                const f32x4 de = *reinterpret_cast<const f32x4*>(a.stat_delta + pr + 8 * g + 4 * h);
+            for (int g = 0; g < KG; ++g) {
+                f32x16 s, dp;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int i = 4 * g + j;
-                    p[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, -ls[j]));
-                    ds[i] = p[i] * (dp[i] - de[j]);
+                for (int i = 0; i < 16; ++i) { s[i] = 0.f; dp[i] = 0.f; }
+                v8 qa = att_row_frag<T, DP>(lq, at, 32 * qb, 0), da = att_row_frag<T, DP>(ld, at, 32 * qb, 0);
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {                  // operands one step ahead and no further: there are no registers for more
+                    v8 qn, dn;
+                    if (ks + 1 < KS) {
+                        qn = att_row_frag<T, DP>(lq, at, 32 * qb, ks + 1);
+                        dn = att_row_frag<T, DP>(ld, at, 32 * qb, ks + 1);
+                    }
+                    if (DP == 128) __builtin_amdgcn_sched_barrier(0);
+                    s = mfma16(qa, kf[g][ks], s);
+                    dp = mfma16(da, vf[g][ks], dp);
+                    if (DP == 128) __builtin_amdgcn_sched_barrier(0);
+                    qa = qn;
+                    da = dn;
                 }
-            }
-            if (!whole) {
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
+                for (int e = 0; e < 4; ++e) {
+                    const f32x4 ls = *reinterpret_cast<const f32x4*>(st + 8 * e);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) s[4 * e + j] = __builtin_amdgcn_exp2f(fmaf(s[4 * e + j], c, -ls[j]));
+                }
+                if (!whole) {
+                    asm volatile("");                              // a branch, not 16 selects in every block
                     typedef int i32x4 __attribute__((ext_vector_type(4)));
-                    const i32x4 lo = *reinterpret_cast<const i32x4*>(a.stat_lo + pr + 8 * g + 4 * h);
-                    const i32x4 hi = *reinterpret_cast<const i32x4*>(a.stat_hi + pr + 8 * g + 4 * h);
+                    const int key = k0 + 32 * g + r;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        if (key < lo[j] || key >= hi[j]) { p[4 * g + j] = 0.f; ds[4 * g + j] = 0.f; }
+                    for (int e = 0; e < 4; ++e) {
+                        const long long pr = pbase + row0 + 8 * e + 4 * h;
+                        const i32x4 lo = *reinterpret_cast<const i32x4*>(a.stat_lo + pr);
+                        const i32x4 hi = *reinterpret_cast<const i32x4*>(a.stat_hi + pr);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            if (key < lo[j] || key >= hi[j]) s[4 * e + j] = 0.f;
+                    }
                 }
+                float p[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) p[i] = s[i];
+#pragma unroll
+                for (int u = 0; u < 2; ++u) pf[g][u] = att_pack<T>(p + 8 * u);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const f32x4 de = *reinterpret_cast<const f32x4*>(st + 64 + 8 * e);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) p[4 * e + j] *= dp[4 * e + j] - de[j];
+                }
+#pragma unroll
+                for (int u = 0; u < 2; ++u) sf[g][u] = att_pack<T>(p + 8 * u);
+                if (DP == 128) __builtin_amdgcn_sched_barrier(0);     // one block of scores at a time in registers
             }
+            v8 da = att_col_frag<T, DP>(ld, at, 32 * qb, 0), qa = att_col_frag<T, DP>(lq, at, 32 * qb, 0);
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const v8 pf = att_pack<T>(p + 8 * u), sf = att_pack<T>(ds + 8 * u);
-#pragma unroll
-                for (int db = 0; db < DB; ++db) {
-                    dv[db] = mfma16(att_col_frag<T, DP>(ld, 32 * qb + 16 * u, db, lane), pf, dv[db]);
-                    dk[db] = mfma16(att_col_frag<T, DP>(lq, 32 * qb + 16 * u, db, lane), sf, dk[db]);
+            for (int i = 0; i < 2 * DB; ++i) {
+                const int u = i / DB, db = i % DB, un = (i + 1) / DB, dn = (i + 1) % DB;
+                v8 dx, qx;
+                if (i + 1 < 2 * DB) {
+                    dx = att_col_frag<T, DP>(ld, at, 32 * qb + 16 * un, dn);
+                    qx = att_col_frag<T, DP>(lq, at, 32 * qb + 16 * un, dn);
                 }
+                if (DP == 128) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int g = 0; g < KG; ++g) {
+                    dv[g][db] = mfma16(da, pf[g][u], dv[g][db]);
+                    dk[g][db] = mfma16(qa, sf[g][u], dk[g][db]);
+                }
+                if (DP == 128) __builtin_amdgcn_sched_barrier(0);
+                da = dx;
+                qa = qx;
             }
         }
     }
-    if (key >= a.M) return;
-    const long long orow = ((long long)b * a.M + key) * a.Hk + hk;
-    if (a.splits > 1) {
-        const long long rows = (long long)a.B * a.M * a.Hk;
-        float* pk = a.part + (split * rows + orow) * a.D;
-        float* pv = pk + (long long)a.splits * rows * a.D;
+    if constexpr (RG == 2) {                                       // the second row group's sums to the first, dK and dV one after the other
+        static_assert(GROUPS * KG * DB * 4096 <= 2 * BUF, "the exchange reuses the tiles");
+#pragma unroll
+        for (int which = 0; which < 2; ++which) {
+            f32x16(&x)[KG][DB] = which ? dv : dk;
+            wg_barrier();
+            float* ex = reinterpret_cast<float*>(smem + kg * KG * DB * 4096);
+#pragma unroll
+            for (int g = 0; g < KG; ++g)
+#pragma unroll
+                for (int db = 0; db < DB; ++db)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        f32x4* at = reinterpret_cast<f32x4*>(ex) + ((g * DB + db) * 4 + e) * 64 + lane;
+                        if (rg == 1) *at = f32x4{x[g][db][4 * e], x[g][db][4 * e + 1], x[g][db][4 * e + 2], x[g][db][4 * e + 3]};
+                    }
+            wg_barrier();
+            if (rg == 0) {
+#pragma unroll
+                for (int g = 0; g < KG; ++g)
+#pragma unroll
+                    for (int db = 0; db < DB; ++db)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const f32x4 v = *(reinterpret_cast<const f32x4*>(ex) + ((g * DB + db) * 4 + e) * 64 + lane);
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) x[g][db][4 * e + j] += v[j];
+                        }
+            }
+        }
+        if (rg == 1) return;
+    }
+#pragma unroll
+    for (int g = 0; g < KG; ++g) {
+        const int key = k0 + 32 * g + r;
+        if (key >= a.M) continue;
+        const long long orow = ((long long)b * a.M + key) * a.Hk + hk;
+        if (a.splits > 1) {
+            const long long rows = (long long)a.B * a.M * a.Hk;
+            float* pk = a.part + (split * rows + orow) * a.D;
+            float* pv = pk + (long long)a.splits * rows * a.D;
+#pragma unroll
+            for (int db = 0; db < DB; ++db) {
+                att_store_block_f32(pk, 32 * db, h, a.D, dk[g][db]);
+                att_store_block_f32(pv, 32 * db, h, a.D, dv[g][db]);
+            }
+            continue;
+        }
+        T* ok = (T*)a.dk + orow * a.D;
+        T* ov = (T*)a.dv + orow * a.D;
 #pragma unroll
         for (int db = 0; db < DB; ++db) {
-            att_store_block_f32(pk, 32 * db, h, a.D, dk[db]);
-            att_store_block_f32(pv, 32 * db, h, a.D, dv[db]);
+            att_store_block<T>(ok, 32 * db, h, a.D, dk[g][db], a.scale);
+            att_store_block<T>(ov, 32 * db, h, a.D, dv[g][db], 1.f);
         }
-        return;
-    }
-    T* ok = (T*)a.dk + orow * a.D;
-    T* ov = (T*)a.dv + orow * a.D;
-#pragma unroll
-    for (int db = 0; db < DB; ++db) {
-        att_store_block<T>(ok, 32 * db, h, a.D, dk[db], a.scale);
-        att_store_block<T>(ov, 32 * db, h, a.D, dv[db], 1.f);
     }
 }
 
@@ -371,7 +462,19 @@ static AttBwdPlan attention_bwd_plan(int B, int N, int M, int H, int Hk, int D) 
         return s < 1 ? 1 : (int)s;
     };
     p.q_splits = pick(pairs * p.q_tiles, (M + 63) / 64);
-    p.k_splits = pick(pairs * p.k_tiles, (rows + 63) / 64);
+    // dK / dV: the split that is done first by a model of workgroups that all see every row, in microseconds: rounds of 64-row steps
+    // (1.3 at DP = 128 with one workgroup per CU, about the same for two of the smaller sizes) plus the partial sums' way to memory
+    // and back at 4 TB/s. (In causal order the tiles differ; the longest go first, and a split halves the longest.)
+    {
+        const long long wgs = pairs * p.k_tiles, slots = 2LL * svps_num_cus(), steps = (rows + 63) / 64;
+        double best = 0.0;
+        p.k_splits = 1;
+        for (int s = 1; s <= 32 && (s == 1 || steps / s >= 4); ++s) {
+            const double t = (double)((wgs * s + slots - 1) / slots) * (double)((steps + s - 1) / s) * 1.3 +
+                             (s > 1 ? 5.0 + (double)s * B * M * Hk * D * 16.0 / 4e6 : 0.0);
+            if (s == 1 || t < best) { best = t; p.k_splits = s; }
+        }
+    }
     p.stat_bytes = (size_t)pairs * p.rows_pad * 4 * sizeof(float);
     const size_t a = p.q_splits > 1 ? (size_t)p.q_splits * B * N * H * D * sizeof(float) : 0;
     const size_t c = p.k_splits > 1 ? (size_t)p.k_splits * B * M * Hk * D * 2 * sizeof(float) : 0;
@@ -382,9 +485,9 @@ static AttBwdPlan attention_bwd_plan(int B, int N, int M, int H, int Hk, int D) 
 template <typename T, int DP>
 static int attention_bwd_launch(AttArgs a, const AttBwdPlan& p, hipStream_t stream) {
     static SvpsLdsAttr attr_q, attr_k;
-    constexpr int KT = 64, QT = 64, LDS = 4 * 64 * DP * 2;
-    hipError_t e = attr_q.ensure((const void*)att_dq_kernel<T, DP, KT>, LDS);
-    if (e == hipSuccess) e = attr_k.ensure((const void*)att_dkdv_kernel<T, DP, QT>, LDS);
+    constexpr int KT = 64, KG = 1, RG = KG, LDS_Q = 4 * KT * DP * 2, LDS_K = 2 * (2 * 64 * DP * 2 + 512);
+    hipError_t e = attr_q.ensure((const void*)att_dq_kernel<T, DP, KT>, LDS_Q);
+    if (e == hipSuccess) e = attr_k.ensure((const void*)att_dkdv_kernel<T, DP, KG, RG>, LDS_K);
     if (e != hipSuccess) return (int)e;
     const long long pairs = (long long)a.B * a.Hk;
     const long long lanes = pairs * a.rows_pad * (DP / 8);
@@ -394,7 +497,7 @@ static int attention_bwd_launch(AttArgs a, const AttBwdPlan& p, hipStream_t stre
     AttArgs k = a;
     k.tiles = p.k_tiles;
     k.splits = p.k_splits;
-    hipLaunchKernelGGL((att_dkdv_kernel<T, DP, QT>), dim3((unsigned)(pairs * k.tiles * k.splits)), dim3(256), LDS, stream, k);
+    hipLaunchKernelGGL((att_dkdv_kernel<T, DP, KG, RG>), dim3((unsigned)(pairs * k.tiles * k.splits)), dim3(256), LDS_K, stream, k);
     e = hipGetLastError();
     if (e != hipSuccess) return (int)e;
     if (k.splits > 1) {
@@ -408,7 +511,7 @@ static int attention_bwd_launch(AttArgs a, const AttBwdPlan& p, hipStream_t stre
     AttArgs q = a;
     q.tiles = p.q_tiles;
     q.splits = p.q_splits;
-    hipLaunchKernelGGL((att_dq_kernel<T, DP, KT>), dim3((unsigned)(pairs * q.tiles * q.splits)), dim3(256), LDS, stream, q);
+    hipLaunchKernelGGL((att_dq_kernel<T, DP, KT>), dim3((unsigned)(pairs * q.tiles * q.splits)), dim3(256), LDS_Q, stream, q);
     e = hipGetLastError();
     if (e != hipSuccess) return (int)e;
     if (q.splits > 1) {

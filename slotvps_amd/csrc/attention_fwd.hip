@@ -80,13 +80,13 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void attention_fwd_kernel
         }
     }
 
-    const char* kbase = (const char*)((const T*)a.k + b * a.skb + hk * a.skh);
-    const char* vbase = (const char*)((const T*)a.v + b * a.svb + hk * a.svh);
-    auto stage = [&](int tile, int buf) {
+    AttTile<DP, KT, NW> tk, tv;
+    tk.init((const T*)a.k + b * a.skb + hk * a.skh, a.skn, 0, a, 1, w, lane);
+    tv.init((const T*)a.v + b * a.svb + hk * a.svh, a.svn, 0, a, 1, w, lane);
+    auto stage = [&](int tile, int buf) __attribute__((always_inline)) {
         char* lk = smem + buf * 2 * TILE;
-        const int k0 = tile * KT;
-        att_stage<DP, KT, NW>(lk, w, lane, a.D, [&](int rr) { const int key = k0 + rr; return key < klen ? kbase + (long long)key * a.skn * 2 : nullptr; });
-        att_stage<DP, KT, NW>(lk + TILE, w, lane, a.D, [&](int rr) { const int key = k0 + rr; return key < klen ? vbase + (long long)key * a.svn * 2 : nullptr; });
+        tk.stage(a, 1, tile, klen, lk, w, lane);
+        tv.stage(a, 1, tile, klen, lk + TILE, w, lane);
     };
 
     f32x16 acc[DB];
@@ -95,7 +95,8 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void attention_fwd_kernel
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[db][i] = 0.f;
     const float c = a.scale * kLog2e;
-    float m = -INFINITY, l = 0.f;                                  // running maximum of q . k and sum of exponentials (this lane half's keys)
+    AttLane<DP> at(lane);
+    float mc = kAttFloor, l = 0.f;                                 // reference point of the exponentials (base 2) and their sum (this lane half's keys)
 
     if (tb < te) stage(tb, 0);
     for (int tile = tb; tile < te; ++tile) {
@@ -107,6 +108,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void attention_fwd_kernel
         if (!wave_on || k0 >= hi_max || k0 + KT <= lo_min) continue;
         const char* lk = smem + buf * 2 * TILE;
         const char* lv = lk + TILE;
+        at.pin();
         float p[KB * 16];
         float mt = -INFINITY;
         const bool whole = k0 >= lo_max && k0 + KT <= hi_min;
@@ -116,11 +118,12 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void attention_fwd_kernel
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[i] = 0.f;
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) s = mfma16(att_row_frag<T, DP>(lk, 32 * kb + r, ks, h), qf[ks], s);
+            for (int ks = 0; ks < KS; ++ks) s = mfma16(att_row_frag<T, DP>(lk, at, 32 * kb, ks), qf[ks], s);
 #pragma unroll
             for (int i = 0; i < 16; ++i) p[16 * kb + i] = s[i];
         }
         if (!whole) {
+            asm volatile("");                                      // a branch, not 32 selects in every tile
 #pragma unroll
             for (int i = 0; i < KB * 16; ++i) {
                 const int key = k0 + 32 * (i >> 4) + acc_row(i & 15, h);
@@ -130,31 +133,32 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void attention_fwd_kernel
 #pragma unroll
         for (int i = 0; i < KB * 16; ++i) mt = fmaxf(mt, p[i]);
         mt = wave_half_xor_max(mt);
-        const float mn = fmaxf(m, mt);
-        const float mc = mn == -INFINITY ? 0.f : mn * c;
-        const float alpha = exp2f(m * c - mc);
-        m = mn;
-        float lt = 0.f;
+        // The reference point of the exponentials moves only when a row's maximum has outgrown it by a factor of 2^8: until then the sums
+        // stay within 2^8 of their scale, and the rescaling (every accumulator of the wave) is skipped.
+        if (__any(mt * c > mc + 8.f)) {
+            const float mn = fmaxf(mc, mt * c);
+            const float alpha = __builtin_amdgcn_exp2f(mc - mn);
+            mc = mn;
+            l *= alpha;
+#pragma unroll
+            for (int db = 0; db < DB; ++db)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[db][i] *= alpha;
+        }
 #pragma unroll
         for (int i = 0; i < KB * 16; ++i) {
             p[i] = __builtin_amdgcn_exp2f(fmaf(p[i], c, -mc));
-            lt += p[i];
+            l += p[i];                                             // before its rounding: the backward pass divides by this sum
         }
-        l = l * alpha + lt;
-#pragma unroll
-        for (int db = 0; db < DB; ++db)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) acc[db][i] *= alpha;
 #pragma unroll
         for (int ks = 0; ks < KT / 16; ++ks) {
             const v8 pf = att_pack<T>(p + 8 * ks);
 #pragma unroll
-            for (int db = 0; db < DB; ++db) acc[db] = mfma16(att_col_frag<T, DP>(lv, 16 * ks, db, lane), pf, acc[db]);
+            for (int db = 0; db < DB; ++db) acc[db] = mfma16(att_col_frag<T, DP>(lv, at, 16 * ks, db), pf, acc[db]);
         }
     }
 
     l = wave_half_xor_sum(l);
-    const float mc = m == -INFINITY ? 0.f : m * c;
     if (n >= a.N) return;
     if (a.splits > 1) {
         const long long rows = (long long)a.B * a.N * a.H;

@@ -42,6 +42,7 @@ template <int BYTES> __device__ __forceinline__ int lin_swz(int row) {      // r
 template <int R, int NW, bool KM>
 struct LinTile {
     static constexpr int LROWS = KM ? 64 : R, BYTES = KM ? R * 2 : 128, CH = BYTES / 16, RPP = 64 / CH, PIECES = LROWS / RPP, N = PIECES / NW;
+    static_assert((CH & (CH - 1)) == 0 && CH <= 64, "the chunk swizzle permutes a power of two of chunks");
     static_assert(PIECES % NW == 0, "every wave stages the same number of pieces");
     const char* base;                           // of the tile at k = 0
     long long step;                             // bytes per step
@@ -61,7 +62,7 @@ struct LinTile {
         const char* b = base + s * step;
         if ((s + 1) * 64 <= K) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) dma16(b + off[i], lds + (i * NW + w) * 1024);
+            for (int i = 0; i < N; ++i) dma_off(dma_base(b), off[i], lds + (i * NW + w) * 1024);
         } else {
 #pragma unroll
             for (int i = 0; i < N; ++i) {
@@ -189,7 +190,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_kernel(LinArgs a) {
     LinTile<BN, NW, WK> tw;
     tx.init(a.x, a.ldx, m0, a.M, w, lane);
     tw.init(a.w, a.ldw, n0, a.N, w, lane);
-    auto stage = [&](int s) {
+    auto stage = [&](int s) __attribute__((always_inline)) {
         char* l = smem + ((s - sb) & 1) * (XB + WB);
         tx.stage(s, a.K, l, w, lane);
         tw.stage(s, a.K, l + XB, w, lane);
@@ -205,18 +206,22 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_kernel(LinArgs a) {
     // tile is in registers, so the tile after next may overwrite it, the next one has had a step to arrive, and its first fragments are
     // read under the last products.
     v8 xf[2][MI], wf[2][NI];
-    auto fetch = [&](int s, int ks, int to) {
+    auto fetch = [&](int s, int ks, int to) __attribute__((always_inline)) {
         const char* lx = smem + ((s - sb) & 1) * (XB + WB);
 #pragma unroll
         for (int i = 0; i < MI; ++i) xf[to][i] = lin_frag<T, BM, XK>(lx, (wm * MI + i) * 32, ks, lane);
 #pragma unroll
         for (int j = 0; j < NI; ++j) wf[to][j] = lin_frag<T, BN, WK>(lx + XB, (wn * NI + j) * 32, ks, lane);
     };
-    auto multiply = [&](int from) {
+    // the scheduling fences keep the reads in front of the products that do not need them (left alone, the compiler sinks every read to
+    // just before its use and waits for it there)
+    auto multiply = [&](int from) __attribute__((always_inline)) {
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < MI; ++i)
 #pragma unroll
             for (int j = 0; j < NI; ++j) acc[i][j] = mfma16(wf[from][j], xf[from][i], acc[i][j]);
+        __builtin_amdgcn_sched_barrier(0);
     };
     if (sb < se) {
         stage(sb);
@@ -462,7 +467,7 @@ static int linear_pack(const void* src, long long ld, void* dst, int rows, int c
 static bool linear_shape_ok(int M, int K, int N, long long ldx, long long ldw) {
     const long long big = 1LL << 30;
     // 256 rows of an operand stay inside 32-bit offsets
-    if (M <= 0 || K <= 0 || N <= 0 || M > big || K > 1 << 22 || N > 1 << 22 || ldx < K || ldw < K || ldx > 1 << 22 || ldw > 1 << 22) return false;
+    if (M <= 0 || K <= 0 || N <= 0 || M > big || K >= 1 << 22 || N >= 1 << 22 || ldx < K || ldw < K || ldx >= 1 << 22 || ldw >= 1 << 22) return false;
     // workgroups, packed rows and 8-element groups of every launch fit 31 bits
     return ((M + 127LL) / 128) * ((N + 127LL) / 128) <= big / 64 && ((M + 127LL) / 128) * ((K + 127LL) / 128) <= big / 64 &&
            ((K + 127LL) / 128) * ((N + 127LL) / 128) <= big / 64;
@@ -588,7 +593,7 @@ static int linear_bwd_t(const T* dy, long long ldy, const T* x, long long ldx, c
 extern "C" size_t svps_linear_act_bwd_workspace_bytes(int M, int K, int N, long long ldy, long long ldx, long long ldw, int unaligned, int has_gate,
                                                       int want_dx, int want_dw, int want_db) {
     using namespace svps;
-    if (!linear_shape_ok(M, K, N, ldx, ldw) || ldy < N || ldy > 1 << 22) return 0;
+    if (!linear_shape_ok(M, K, N, ldx, ldw) || ldy < N || ldy >= 1 << 22) return 0;
     const LinBwdPlan p = linear_bwd_plan(M, K, N, has_gate || unaligned || (ldy & 7) || (N & 7), unaligned || (ldx & 7) || (K & 7),
                                          unaligned || (ldw & 7) || (K & 7), want_dx, want_dw, want_db);
     return p.dz + p.x + p.w + p.sums + p.part;
@@ -600,7 +605,7 @@ extern "C" int svps_linear_act_bwd(const void* dy, long long ldy, const void* x,
     using namespace svps;
     if (!dy || (!dx && !dw && !db) || (dx && !w) || (dw && !x)) return SVPS_ERR_BAD_ARG;
     if (dtype != SVPS_DTYPE_BF16 && dtype != SVPS_DTYPE_F16) return SVPS_ERR_BAD_ARG;
-    if (!linear_shape_ok(M, K, N, x ? ldx : K, w ? ldw : K) || ldy < N || ldy > 1 << 22) return SVPS_ERR_BAD_SHAPE;
+    if (!linear_shape_ok(M, K, N, x ? ldx : K, w ? ldw : K) || ldy < N || ldy >= 1 << 22) return SVPS_ERR_BAD_SHAPE;
     if ((M + kDzRows - 1) / kDzRows > 65535) return SVPS_ERR_BAD_SHAPE;
     const LinBwdPlan p = linear_bwd_plan(M, K, N, (dx || dw) && (gate || !lin_direct(dy, ldy, N)), !lin_direct(x, ldx, K), !lin_direct(w, ldw, K),
                                          dx != nullptr, dw != nullptr, db != nullptr);

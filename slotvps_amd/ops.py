@@ -1404,7 +1404,7 @@ def _rows16(t, name, dtype, cols):
     """[..., cols] -> 2-D rows with contiguous columns and a row stride >= cols (a view where that is possible)."""
     t = _token_tensor(t, name, (dtype,))
     t = t.reshape(-1, cols)
-    if (cols > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and not cols <= t.stride(0) <= 1 << 22):
+    if (cols > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and not cols <= t.stride(0) < 1 << 22):
         t = t.contiguous()
     return t
 
@@ -1420,8 +1420,8 @@ def _linear_args(x, weight, bias, act, residual):
     N, K = weight.shape
     if x.shape[-1] != K or K == 0:
         raise ValueError(f"linear_act: x {tuple(x.shape)} does not match weight {tuple(weight.shape)}")
-    if max(K, N) > 1 << 22:
-        raise ValueError("linear_act: at most 2^22 channels on either side")
+    if max(K, N) >= 1 << 22:
+        raise ValueError("linear_act: fewer than 2^22 channels on either side")
     weight = _rows16(weight, "weight", x.dtype, K)
     if act not in (ACT_NONE, ACT_RELU, ACT_GELU):
         raise ValueError("linear_act: act must be ACT_NONE, ACT_RELU or ACT_GELU")
