@@ -60,7 +60,7 @@ __global__ __launch_bounds__(256, 2) void att_dq_kernel(AttArgs a) {
     const int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int pairs = a.B * a.Hk;
-    const int id = blockIdx.x, pair = id % pairs, rest = id / pairs;
+    const int id = blockIdx.x, rest = id / pairs, pair = att_pair(id, rest, pairs);
     const int t = a.tiles - 1 - rest % a.tiles, split = rest / a.tiles;
     const int b = pair / a.Hk, hk = pair - b * a.Hk;
     const int qlen = att_qlen(a, b), klen = att_klen(a, b);
@@ -196,7 +196,7 @@ __global__ __launch_bounds__(256, 2) void att_dkdv_kernel(AttArgs a) {
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int kg = w % GROUPS, rg = w / GROUPS;
     const int pairs = a.B * a.Hk;
-    const int id = blockIdx.x, pair = id % pairs, rest = id / pairs;
+    const int id = blockIdx.x, rest = id / pairs, pair = att_pair(id, rest, pairs);
     const int t = rest / a.splits, split = rest - t * a.splits;    // early keys are seen by the most rows: longest first
     const int b = pair / a.Hk, hk = pair - b * a.Hk;
     const int qlen = att_qlen(a, b), klen = att_klen(a, b);

@@ -18,8 +18,8 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void attention_fwd_kernel
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int pairs = a.B * a.Hk;
     const int id = blockIdx.x;
-    const int pair = id % pairs;                                   // 8 | pairs: a pair's tiles meet on one XCD and share its L2
     const int rest = id / pairs;
+    const int pair = att_pair(id, rest, pairs);
     const int t = a.tiles - 1 - rest % a.tiles;                    // late rows see the most keys in causal order: longest first
     const int split = rest / a.tiles;
     const int b = pair / a.Hk, hk = pair - b * a.Hk;
@@ -132,11 +132,10 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void attention_fwd_kernel
         }
 #pragma unroll
         for (int i = 0; i < KB * 16; ++i) mt = fmaxf(mt, p[i]);
-        mt = wave_half_xor_max(mt);
         // The reference point of the exponentials moves only when a row's maximum has outgrown it by a factor of 2^8: until then the sums
         // stay within 2^8 of their scale, and the rescaling (every accumulator of the wave) is skipped.
         if (__any(mt * c > mc + 8.f)) {
-            const float mn = fmaxf(mc, mt * c);
+            const float mn = fmaxf(mc, wave_half_xor_max(mt) * c);     // a row's keys are in both lane halves: one point for both
             const float alpha = __builtin_amdgcn_exp2f(mc - mn);
             mc = mn;
             l *= alpha;
