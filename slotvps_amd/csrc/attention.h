@@ -31,12 +31,28 @@ struct AttArgs {
     float* lse;                                 // [B, H, N]
     long long sqb, sqn, sqh, skb, skn, skh, svb, svn, svh, sdb, sdn, sdh;
     const int* qlens; const int* klens;
-    float* part;                                // partial sums of splits
+    float* part; float* k_part;                 // partial sums of splits (backward: dQ | dK, dV)
     float* stat_lse2; float* stat_delta; int* stat_lo; int* stat_hi;   // backward: per packed row, [B * Hk][rows_pad]
-    int B, N, M, H, Hk, G, D, frame, window, splits, tiles, rows_pad;
+    int B, N, M, H, Hk, G, D, frame, window, splits, tiles, k_splits, k_tiles, rows_pad;
     unsigned gmagic;                            // floor(2^32 / G) + 1
     float scale;
 };
+
+// the lane's number, computed where it stands (a value kept from the start would hold a register through the main loop)
+__device__ __forceinline__ int att_lane() {
+    int x;
+    asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(x));
+    return x;
+}
+
+// The kernel's arguments (its only parameter) read again from memory: for code behind or beside the main loop, whose values would otherwise
+// stand in scalar registers all through it (and push each other out of them).
+typedef const AttArgs __attribute__((address_space(4))) AttArgsMem;
+__device__ __forceinline__ AttArgsMem* att_args() {
+    AttArgsMem* p = (AttArgsMem*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return p;
+}
 
 __device__ __forceinline__ int att_qlen(const AttArgs& a, int b) {
     if (!a.qlens) return a.N;
@@ -50,7 +66,8 @@ __device__ __forceinline__ int att_klen(const AttArgs& a, int b) {
 }
 
 // row / G without a division: the product with floor(2^32 / G) + 1 is never short and at most one too far
-__device__ __forceinline__ int att_div_g(const AttArgs& a, int row) {
+template <typename A>
+__device__ __forceinline__ int att_div_g(const A& a, int row) {
     if (a.G == 1) return row;
     int n = (int)__umulhi((unsigned)row, a.gmagic);
     return n - ((long long)n * a.G > row ? 1 : 0);
@@ -89,15 +106,31 @@ template <int DP> __device__ __forceinline__ int att_swz(int row) {
 
 static __device__ __attribute__((aligned(16))) uint32_t g_att_zero[4];       // never written: the source of padded rows and channels
 
-// LDS-DMA with a wave-uniform base (64-bit, in scalar registers) and a 32-bit lane offset below 2 GiB: no vector arithmetic, one register
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t dma_base(const char* base) {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, 0x7fffffff, 0x00027000);
+// LDS-DMA: 64 lanes x 16 (4) bytes to lds_base + lane * 16 (4), with a wave-uniform base (64-bit, scalar registers) and a 32-bit lane offset
+// below 2 GiB, or with a 64-bit address per lane. Written as instructions: behind the builtin the compiler knows of a pending write to LDS
+// and waits for ALL of them in front of every transposed read, i.e. for the tile it has just asked for. Nothing is returned to a register;
+// the waits are the ones in the code (wait_vm in front of the barrier that hands a tile over).
+__device__ __forceinline__ uint32_t lds_address(const char* p) {
+    return __builtin_amdgcn_readfirstlane((uint32_t)reinterpret_cast<uintptr_t>(p));        // the low half of a flat address into LDS
 }
-__device__ __forceinline__ void dma_off(__amdgpu_buffer_rsrc_t base, uint32_t lane_off, char* lds_base) {          // 16 bytes per lane
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(base, (SVPS_LDS void*)lds_base, 16, lane_off, 0, 0, 0);
+__device__ __forceinline__ u32x4 dma_base(const char* base) {
+    const uint64_t a = reinterpret_cast<uint64_t>(base);
+    return u32x4{(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)a), (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(a >> 32) & 0xffffu), 0x7fffffffu, 0x00020000u};
 }
-__device__ __forceinline__ void dma_off4(__amdgpu_buffer_rsrc_t base, uint32_t lane_off, char* lds_base) {         // 4 bytes per lane
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(base, (SVPS_LDS void*)lds_base, 4, lane_off, 0, 0, 0);
+__device__ __forceinline__ void dma_off(u32x4 base, uint32_t lane_off, const char* lds_base) {
+    uint32_t keep;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, 0 offen lds\n\ts_mov_b32 m0, %0"
+                 : "=&s"(keep) : "s"(lds_address(lds_base)), "v"(lane_off), "s"(base) : "memory");
+}
+__device__ __forceinline__ void dma_off4(u32x4 base, uint32_t lane_off, const char* lds_base) {
+    uint32_t keep;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dword %2, %3, 0 offen lds\n\ts_mov_b32 m0, %0"
+                 : "=&s"(keep) : "s"(lds_address(lds_base)), "v"(lane_off), "s"(base) : "memory");
+}
+__device__ __forceinline__ void dma_ptr(const char* src, const char* lds_base) {
+    uint32_t keep;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off\n\ts_mov_b32 m0, %0"
+                 : "=&s"(keep) : "s"(lds_address(lds_base)), "v"(src) : "memory");
 }
 
 template <typename T> struct AttVec;
@@ -108,19 +141,23 @@ template <> struct AttVec<_Float16> { typedef f16x8 v8; typedef f16x4 v4; };
 // group (keys and values: G = 1). For whole tiles of DP channels a lane's offsets are the same in every tile and only the wave-uniform
 // base moves (no address arithmetic in the loop); rows behind the last valid one and padded channels take zeros on a slower path - what
 // stands behind a length must not reach a product, 0 * NaN included.
-template <int DP, int ROWS, int NW>
+enum { kAttQ, kAttK, kAttV, kAttDout };
+template <int DP, int ROWS, int NW, int OP>
 struct AttTile {
     static constexpr int CH = DP / 8, RPP = 64 / CH, PIECES = ROWS / RPP, N = PIECES / NW, LEAP = RPP * NW;
     static constexpr int NOFF = LEAP % 16 == 0 ? 1 : N;     // pieces 16 k rows apart have the same swizzle: one offset, the rest is uniform
     static_assert(PIECES % NW == 0, "every wave stages the same number of pieces");
     const char* base;
-    long long sn, sh, step, leap;               // bytes: token, head, tile, piece
+    long long step, leap;                       // bytes from tile to tile, from piece to piece
     uint32_t off[NOFF];
     bool quick;
-    __device__ __forceinline__ void init(const void* p, long long token, long long head, const AttArgs& a, int G, int w, int lane) {
+    template <typename A> static __device__ __forceinline__ long long token(const A& a) { return 2 * (OP == kAttQ ? a.sqn : OP == kAttK ? a.skn : OP == kAttV ? a.svn : a.sdn); }
+    template <typename A> static __device__ __forceinline__ long long head(const A& a) { return OP == kAttQ ? 2 * a.sqh : OP == kAttDout ? 2 * a.sdh : 0; }
+    template <typename A> static __device__ __forceinline__ int group(const A& a) { return OP == kAttQ || OP == kAttDout ? a.G : 1; }
+    __device__ __forceinline__ void init(const void* p, const AttArgs& a, int w, int lane) {
+        const long long sn = token(a), sh = head(a);
+        const int G = group(a);
         base = (const char*)p;
-        sn = token * 2;
-        sh = head * 2;
         step = sn * (ROWS / G);
         leap = NOFF == 1 ? sn * (LEAP / G) : 0;
         quick = a.D == DP && ROWS % G == 0 && (NOFF > 1 || LEAP % G == 0) && (unsigned long long)(step + sh * G) < 0x80000000ULL;
@@ -131,20 +168,21 @@ struct AttTile {
         }
     }
     // tile number `tile` of `rows` valid packed rows
-    __device__ __forceinline__ void stage(const AttArgs& a, int G, int tile, int rows, char* lds, int w, int lane) const {
+    __device__ __forceinline__ void stage(int tile, int rows, char* lds, int w, int lane) const {
         if (quick && (tile + 1) * ROWS <= rows) {
             const char* b = base + tile * step;
 #pragma unroll
             for (int i = 0; i < N; ++i) dma_off(dma_base(b + i * leap), off[NOFF == 1 ? 0 : i], lds + (i * NW + w) * 1024);
             return;
         }
+        AttArgsMem& a = *att_args();
 #pragma unroll 1
         for (int i = 0; i < N; ++i) {
             const int lr = (i * NW + w) * RPP + lane / CH, row = tile * ROWS + lr;
             const int chunk = (lane % CH) ^ att_swz<DP>(lr);
-            const int n = G == 1 ? row : att_div_g(a, row);
-            const char* p = base + n * sn + (row - n * G) * sh + chunk * 16;
-            dma16(row < rows && chunk * 8 < a.D ? p : reinterpret_cast<const char*>(g_att_zero), lds + (i * NW + w) * 1024);
+            const int n = group(a) == 1 ? row : att_div_g(a, row);
+            const char* p = base + n * token(a) + (row - n * group(a)) * head(a) + chunk * 16;
+            dma_ptr(row < rows && chunk * 8 < a.D ? p : reinterpret_cast<const char*>(g_att_zero), lds + (i * NW + w) * 1024);
         }
     }
 };

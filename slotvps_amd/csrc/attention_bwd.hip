@@ -1,10 +1,10 @@
 // Attention backward (attention.h has the layouts): the probabilities are computed again from q, k and the forward's log-sum-exp,
 //   p = exp(s - lse),  delta_i = sum_d dO_id O_id,  dV = P^T dO,  dS = P * (dO V^T - delta),  dQ = scale dS K,  dK = scale dS^T Q.
 //
-// Three launches, no atomics, every sum in a fixed order:
-//   att_stats_kernel    per packed row: lse in base 2, delta, visible interval - contiguous, so that the next two read them as vectors
-//   att_dkdv_kernel     a wave owns 32 keys (k, v as operand fragments in registers), walks over the rows that see them (q, dO in LDS)
-//   att_dq_kernel       a wave owns 32 rows, walks over their keys like the forward
+// Two launches, no atomics, every sum in a fixed order:
+//   att_stats_kernel    per packed row: lse in base 2, delta, visible interval - contiguous, so that the next one reads them as vectors
+//   att_bwd_kernel      att_dkdv: a wave owns 32 keys (k, v as operand fragments in registers), walks over the rows that see them (q, dO
+//                       in LDS);  att_dq: a wave owns 32 rows, walks over their keys like the forward
 // That is 7 matrix products for the 5 of one joint kernel; the joint form would add dQ from many workgroups with atomics, whose order
 // changes the result, or write every dS to memory (2 bytes per visible pair and head).
 // Few tiles on either side: the walked range is split over workgroups that leave fp32 partial sums, added by att_add_kernel.
@@ -52,15 +52,15 @@ __global__ __launch_bounds__(256) void att_stats_kernel(AttArgs a) {
     }
 }
 
-template <typename T, int DP, int KT>
-__global__ __launch_bounds__(256, 2) void att_dq_kernel(AttArgs a) {
+// dQ of 128 packed rows: a wave owns 32 rows and walks over their keys
+template <typename T, int DP>
+__device__ __forceinline__ void att_dq(const AttArgs& a, const int id, char* smem) {
     typedef typename AttVec<T>::v8 v8;
-    constexpr int KS = DP / 16, DB = DP / 32, KB = KT / 32, TILE = KT * DP * 2, NW = 4;
-    extern __shared__ __attribute__((aligned(16))) char smem[];
+    constexpr int KT = 64, KS = DP / 16, DB = DP / 32, KB = KT / 32, TILE = KT * DP * 2, NW = 4;
     const int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int pairs = a.B * a.Hk;
-    const int id = blockIdx.x, rest = id / pairs, pair = att_pair(id, rest, pairs);
+    const int rest = id / pairs, pair = att_pair(id, rest, pairs);
     const int t = a.tiles - 1 - rest % a.tiles, split = rest / a.tiles;
     const int b = pair / a.Hk, hk = pair - b * a.Hk;
     const int qlen = att_qlen(a, b), klen = att_klen(a, b);
@@ -68,7 +68,6 @@ __global__ __launch_bounds__(256, 2) void att_dq_kernel(AttArgs a) {
     const int n = att_div_g(a, row);
     const int head = hk * a.G + (row - n * a.G);
     const bool have = n < qlen;
-    const long long orow = ((long long)b * a.N + n) * a.H + head;
     const int wg0 = att_div_g(a, t * NW * 32);
     int wg1 = att_div_g(a, t * NW * 32 + NW * 32 - 1);
     wg1 = wg1 < qlen ? wg1 : qlen - 1;
@@ -111,13 +110,14 @@ __global__ __launch_bounds__(256, 2) void att_dq_kernel(AttArgs a) {
             df[ks] = __builtin_bit_cast(v8, y);
         }
     }
-    AttTile<DP, KT, NW> tk, tv;
-    tk.init((const T*)a.k + b * a.skb + hk * a.skh, a.skn, 0, a, 1, w, lane);
-    tv.init((const T*)a.v + b * a.svb + hk * a.svh, a.svn, 0, a, 1, w, lane);
+    AttTile<DP, KT, NW, kAttK> tk;
+    AttTile<DP, KT, NW, kAttV> tv;
+    tk.init((const T*)a.k + b * a.skb + hk * a.skh, a, w, lane);
+    tv.init((const T*)a.v + b * a.svb + hk * a.svh, a, w, lane);
     auto stage = [&](int tile, int buf) __attribute__((always_inline)) {
         char* lk = smem + buf * 2 * TILE;
-        tk.stage(a, 1, tile, klen, lk, w, lane);
-        tv.stage(a, 1, tile, klen, lk + TILE, w, lane);
+        tk.stage(tile, klen, lk, w, lane);
+        tv.stage(tile, klen, lk + TILE, w, lane);
     };
     f32x16 acc[DB];
 #pragma unroll
@@ -170,37 +170,35 @@ __global__ __launch_bounds__(256, 2) void att_dq_kernel(AttArgs a) {
             }
         }
     }
-    if (n >= a.N) return;
-    if (a.splits > 1) {
-        float* po = a.part + (split * ((long long)a.B * a.N * a.H) + orow) * a.D;
+    AttArgsMem& m = *att_args();
+    if (n >= m.N) return;
+    const long long orow = ((long long)b * m.N + n) * m.H + hk * m.G + (row - n * m.G);
+    if (m.splits > 1) {
+        float* po = m.part + (split * ((long long)m.B * m.N * m.H) + orow) * m.D;
 #pragma unroll
-        for (int db = 0; db < DB; ++db) att_store_block_f32(po, 32 * db, h, a.D, acc[db]);
+        for (int db = 0; db < DB; ++db) att_store_block_f32(po, 32 * db, h, m.D, acc[db]);
         return;
     }
-    T* o = (T*)a.dq + orow * a.D;
+    T* o = (T*)m.dq + orow * m.D;
 #pragma unroll
-    for (int db = 0; db < DB; ++db) att_store_block<T>(o, 32 * db, h, a.D, acc[db], a.scale);
+    for (int db = 0; db < DB; ++db) att_store_block<T>(o, 32 * db, h, m.D, acc[db], m.scale);
 }
 
-// dK, dV of 128 keys: KG blocks of 32 keys per wave, RG groups of waves that take turns at the row blocks (4 / RG groups of keys).
-//   DP <= 64: KG = 1, RG = 1, two waves per SIMD hide each other's waits (the exponentials bound it)
-//   DP = 128: KG = 2, RG = 2: a fragment read from LDS serves two products (with one, LDS reads and products would take the same time and
-//   neither would run at its rate); 128 + 256 registers of operands and sums leave one wave per SIMD, the two row groups add up at the end
-// (lse, delta) of a tile's rows come by LDS-DMA with the rows.
-template <typename T, int DP, int KG, int RG>
-__global__ __launch_bounds__(256, 2) void att_dkdv_kernel(AttArgs a) {
+// dK, dV of 128 keys: a wave owns 32 keys, their k and v stay in registers as operand fragments (at DP = 128 the sums and they are 192 of 256
+// registers: one block of scores at a time, fragments one step ahead, two of v's eight fragments in LDS - with all in registers a few
+// values went to scratch, whose loads stand in one queue with the tiles on their way). (lse, delta) of a tile's rows come by LDS-DMA with the rows.
+template <typename T, int DP>
+__device__ __forceinline__ void att_dkdv(const AttArgs& a, const int id, char* smem) {
     typedef typename AttVec<T>::v8 v8;
-    constexpr int KS = DP / 16, DB = DP / 32, QT = 64, TILE = QT * DP * 2, NW = 4, BUF = 2 * TILE + 512, GROUPS = NW / RG;
-    extern __shared__ __attribute__((aligned(16))) char smem[];
+    constexpr int KS = DP / 16, DB = DP / 32, QT = 64, TILE = QT * DP * 2, NW = 4, BUF = 2 * TILE + 512, VR = DP == 128 ? 6 : KS;
     const int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int kg = w % GROUPS, rg = w / GROUPS;
     const int pairs = a.B * a.Hk;
-    const int id = blockIdx.x, rest = id / pairs, pair = att_pair(id, rest, pairs);
-    const int t = rest / a.splits, split = rest - t * a.splits;    // early keys are seen by the most rows: longest first
+    const int rest = id / pairs, pair = att_pair(id, rest, pairs);
+    const int t = rest / a.k_splits, split = rest - t * a.k_splits;    // early keys are seen by the most rows: longest first
     const int b = pair / a.Hk, hk = pair - b * a.Hk;
     const int qlen = att_qlen(a, b), klen = att_klen(a, b);
-    const int wk0 = t * 128, k0 = wk0 + 32 * KG * kg;
+    const int wk0 = t * 128, k0 = wk0 + 32 * w, key = k0 + r;
 
     // tokens that see a key of [wk0, wk1): their frame is not before the first key's, and not `window` or more behind the last key's
     int n0 = 0, n1 = wk0 < klen ? qlen : 0;
@@ -219,16 +217,15 @@ __global__ __launch_bounds__(256, 2) void att_dkdv_kernel(AttArgs a) {
         tb = (int)((long long)n0 * a.G / QT);
         te = (int)(((long long)n1 * a.G + QT - 1) / QT);
     }
-    if (a.splits > 1) {
-        const int per = (te - tb + a.splits - 1) / a.splits;
+    if (a.k_splits > 1) {
+        const int per = (te - tb + a.k_splits - 1) / a.k_splits;
         tb += split * per;
         te = tb + per < te ? tb + per : te;
     }
 
-    v8 kf[KG][KS], vf[KG][KS];
-#pragma unroll
-    for (int g = 0; g < KG; ++g) {
-        const int key = k0 + 32 * g + r;
+    v8 kf[KS], vf[VR];
+    char* vkeep = smem + 2 * BUF + w * (KS - VR) * 1024 + lane * 16;
+    {
         const T* kp = (const T*)a.k + b * a.skb + hk * a.skh + (long long)key * a.skn;
         const T* vp = (const T*)a.v + b * a.svb + hk * a.svh + (long long)key * a.svn;
 #pragma unroll
@@ -239,30 +236,30 @@ __global__ __launch_bounds__(256, 2) void att_dkdv_kernel(AttArgs a) {
                 x = *reinterpret_cast<const u32x4*>(kp + d);
                 y = *reinterpret_cast<const u32x4*>(vp + d);
             }
-            kf[g][ks] = __builtin_bit_cast(v8, x);
-            vf[g][ks] = __builtin_bit_cast(v8, y);
+            kf[ks] = __builtin_bit_cast(v8, x);
+            if (ks < VR) vf[ks < VR ? ks : 0] = __builtin_bit_cast(v8, y);
+            else *reinterpret_cast<u32x4*>(vkeep + (ks - VR) * 1024) = y;     // read by the lane that wrote it
         }
     }
     const long long pbase = (long long)pair * a.rows_pad;
-    AttTile<DP, QT, NW> tq, td;
-    tq.init((const T*)a.q + b * a.sqb + hk * a.G * a.sqh, a.sqn, a.sqh, a, a.G, w, lane);
-    td.init((const T*)a.dout + b * a.sdb + hk * a.G * a.sdh, a.sdn, a.sdh, a, a.G, w, lane);
+    AttTile<DP, QT, NW, kAttQ> tq;
+    AttTile<DP, QT, NW, kAttDout> td;
+    tq.init((const T*)a.q + b * a.sqb + hk * a.G * a.sqh, a, w, lane);
+    td.init((const T*)a.dout + b * a.sdb + hk * a.G * a.sdh, a, w, lane);
     auto stage = [&](int tile, int buf) __attribute__((always_inline)) {
         char* lq = smem + buf * BUF;
-        tq.stage(a, a.G, tile, qlen * a.G, lq, w, lane);
-        td.stage(a, a.G, tile, qlen * a.G, lq + TILE, w, lane);
+        tq.stage(tile, qlen * a.G, lq, w, lane);
+        td.stage(tile, qlen * a.G, lq + TILE, w, lane);
         if (w < 2) {                                               // 64 rows of lse2 (wave 0) and delta (wave 1); rows_pad is a multiple of 128
             const float* src = (w ? a.stat_delta : a.stat_lse2) + pbase + tile * QT;
-            dma_off4(dma_base((const char*)src), lane * 4, lq + 2 * TILE + 256 * w);
+            dma_off4(dma_base((const char*)src), att_lane() * 4, lq + 2 * TILE + 256 * w);
         }
     };
-    f32x16 dk[KG][DB], dv[KG][DB];
+    f32x16 dk[DB], dv[DB];
 #pragma unroll
-    for (int g = 0; g < KG; ++g)
+    for (int db = 0; db < DB; ++db)
 #pragma unroll
-        for (int db = 0; db < DB; ++db)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) { dk[g][db][i] = 0.f; dv[g][db][i] = 0.f; }
+        for (int i = 0; i < 16; ++i) { dk[db][i] = 0.f; dv[db][i] = 0.f; }
     const float c = a.scale * kLog2e;
     AttLane<DP> at(lane);
     if (tb < te) stage(tb, 0);
@@ -274,78 +271,75 @@ __global__ __launch_bounds__(256, 2) void att_dkdv_kernel(AttArgs a) {
         const char* lq = smem + buf * BUF;
         const char* ld = lq + TILE;
 #pragma unroll 1
-        for (int qb = rg; qb < QT / 32; qb += RG) {
+        for (int qb = 0; qb < QT / 32; ++qb) {
             const int row0 = tile * QT + 32 * qb;
             // interval bounds never fall along the rows: those of the block's first and last token decide whether comparisons are needed, or anything
             const int nf = att_div_g(a, row0), nl = att_div_g(a, row0 + 31);
             if (k0 >= klen || nf >= qlen) continue;
-            bool whole = nl < qlen && k0 + 32 * KG <= klen;
+            bool whole = nl < qlen && k0 + 32 <= klen;
             if (a.frame > 0) {
                 int lo_f, hi_f, lo_l, hi_l;
                 att_range(a, nf, qlen, klen, lo_f, hi_f);
                 att_range(a, nl < qlen ? nl : qlen - 1, qlen, klen, lo_l, hi_l);
-                if (k0 + 32 * KG <= lo_f || k0 >= hi_l) continue;
-                whole = whole && k0 >= lo_l && k0 + 32 * KG <= hi_f;
+                if (k0 + 32 <= lo_f || k0 >= hi_l) continue;
+                whole = whole && k0 >= lo_l && k0 + 32 <= hi_f;
             }
             at.pin();
             const float* st = reinterpret_cast<const float*>(lq + 2 * TILE) + 32 * qb + 4 * h;
-            v8 pf[KG][2], sf[KG][2];
+            v8 pf[2], sf[2];
+            f32x16 s, dp;
 #pragma unroll
-            for (int g = 0; g < KG; ++g) {
-                f32x16 s, dp;
+            for (int i = 0; i < 16; ++i) { s[i] = 0.f; dp[i] = 0.f; }
+            v8 qa = att_row_frag<T, DP>(lq, at, 32 * qb, 0), da = att_row_frag<T, DP>(ld, at, 32 * qb, 0);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) { s[i] = 0.f; dp[i] = 0.f; }
-                v8 qa = att_row_frag<T, DP>(lq, at, 32 * qb, 0), da = att_row_frag<T, DP>(ld, at, 32 * qb, 0);
-#pragma unroll
-                for (int ks = 0; ks < KS; ++ks) {                  // operands one step ahead and no further: there are no registers for more
-                    v8 qn, dn;
-                    if (ks + 1 < KS) {
-                        qn = att_row_frag<T, DP>(lq, at, 32 * qb, ks + 1);
-                        dn = att_row_frag<T, DP>(ld, at, 32 * qb, ks + 1);
-                    }
-                    if (DP == 128) __builtin_amdgcn_sched_barrier(0);
-                    s = mfma16(qa, kf[g][ks], s);
-                    dp = mfma16(da, vf[g][ks], dp);
-                    if (DP == 128) __builtin_amdgcn_sched_barrier(0);
-                    qa = qn;
-                    da = dn;
+            for (int ks = 0; ks < KS; ++ks) {                      // operands one step ahead and no further: at DP = 128 there are no registers for more
+                v8 qn, dn;
+                if (ks + 1 < KS) {
+                    qn = att_row_frag<T, DP>(lq, at, 32 * qb, ks + 1);
+                    dn = att_row_frag<T, DP>(ld, at, 32 * qb, ks + 1);
                 }
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const f32x4 ls = *reinterpret_cast<const f32x4*>(st + 8 * e);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) s[4 * e + j] = __builtin_amdgcn_exp2f(fmaf(s[4 * e + j], c, -ls[j]));
-                }
-                if (!whole) {
-                    asm volatile("");                              // a branch, not 16 selects in every block
-                    typedef int i32x4 __attribute__((ext_vector_type(4)));
-                    const int key = k0 + 32 * g + r;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const long long pr = pbase + row0 + 8 * e + 4 * h;
-                        const i32x4 lo = *reinterpret_cast<const i32x4*>(a.stat_lo + pr);
-                        const i32x4 hi = *reinterpret_cast<const i32x4*>(a.stat_hi + pr);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            if (key < lo[j] || key >= hi[j]) s[4 * e + j] = 0.f;
-                    }
-                }
-                float p[16];
-#pragma unroll
-                for (int i = 0; i < 16; ++i) p[i] = s[i];
-#pragma unroll
-                for (int u = 0; u < 2; ++u) pf[g][u] = att_pack<T>(p + 8 * u);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const f32x4 de = *reinterpret_cast<const f32x4*>(st + 64 + 8 * e);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) p[4 * e + j] *= dp[4 * e + j] - de[j];
-                }
-#pragma unroll
-                for (int u = 0; u < 2; ++u) sf[g][u] = att_pack<T>(p + 8 * u);
-                if (DP == 128) __builtin_amdgcn_sched_barrier(0);     // one block of scores at a time in registers
+                const v8 vv = ks < VR ? vf[ks < VR ? ks : 0] : *reinterpret_cast<const v8*>(vkeep + (ks - VR) * 1024);
+                if (DP == 128) __builtin_amdgcn_sched_barrier(0);
+                s = mfma16(qa, kf[ks], s);
+                dp = mfma16(da, vv, dp);
+                if (DP == 128) __builtin_amdgcn_sched_barrier(0);
+                qa = qn;
+                da = dn;
             }
-            v8 da = att_col_frag<T, DP>(ld, at, 32 * qb, 0), qa = att_col_frag<T, DP>(lq, at, 32 * qb, 0);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const f32x4 ls = *reinterpret_cast<const f32x4*>(st + 8 * e);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) s[4 * e + j] = __builtin_amdgcn_exp2f(fmaf(s[4 * e + j], c, -ls[j]));
+            }
+            if (!whole) {
+                AttArgsMem& m = *att_args();                       // (also keeps this a branch instead of 16 selects in every block)
+                typedef int i32x4 __attribute__((ext_vector_type(4)));
+                const int h4 = (att_lane() >> 5) * 4;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const i32x4 lo = *reinterpret_cast<const i32x4*>(m.stat_lo + pbase + row0 + (8 * e + h4));
+                    const i32x4 hi = *reinterpret_cast<const i32x4*>(m.stat_hi + pbase + row0 + (8 * e + h4));
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (key < lo[j] || key >= hi[j]) s[4 * e + j] = 0.f;
+                }
+            }
+            float p[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) p[i] = s[i];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) pf[u] = att_pack<T>(p + 8 * u);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const f32x4 de = *reinterpret_cast<const f32x4*>(st + 64 + 8 * e);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) p[4 * e + j] *= dp[4 * e + j] - de[j];
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) sf[u] = att_pack<T>(p + 8 * u);
+            if (DP == 128) __builtin_amdgcn_sched_barrier(0);     // one block of scores at a time in registers
+            v8 dc = att_col_frag<T, DP>(ld, at, 32 * qb, 0), qc = att_col_frag<T, DP>(lq, at, 32 * qb, 0);
 #pragma unroll
             for (int i = 0; i < 2 * DB; ++i) {
                 const int u = i / DB, db = i % DB, un = (i + 1) / DB, dn = (i + 1) % DB;
@@ -355,73 +349,44 @@ __global__ __launch_bounds__(256, 2) void att_dkdv_kernel(AttArgs a) {
                     qx = att_col_frag<T, DP>(lq, at, 32 * qb + 16 * un, dn);
                 }
                 if (DP == 128) __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (int g = 0; g < KG; ++g) {
-                    dv[g][db] = mfma16(da, pf[g][u], dv[g][db]);
-                    dk[g][db] = mfma16(qa, sf[g][u], dk[g][db]);
-                }
+                dv[db] = mfma16(dc, pf[u], dv[db]);
+                dk[db] = mfma16(qc, sf[u], dk[db]);
                 if (DP == 128) __builtin_amdgcn_sched_barrier(0);
-                da = dx;
-                qa = qx;
+                dc = dx;
+                qc = qx;
             }
         }
     }
-    if constexpr (RG == 2) {                                       // the second row group's sums to the first, dK and dV one after the other
-        static_assert(GROUPS * KG * DB * 4096 <= 2 * BUF, "the exchange reuses the tiles");
-#pragma unroll
-        for (int which = 0; which < 2; ++which) {
-            f32x16(&x)[KG][DB] = which ? dv : dk;
-            wg_barrier();
-            float* ex = reinterpret_cast<float*>(smem + kg * KG * DB * 4096);
-#pragma unroll
-            for (int g = 0; g < KG; ++g)
-#pragma unroll
-                for (int db = 0; db < DB; ++db)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        f32x4* at = reinterpret_cast<f32x4*>(ex) + ((g * DB + db) * 4 + e) * 64 + lane;
-                        if (rg == 1) *at = f32x4{x[g][db][4 * e], x[g][db][4 * e + 1], x[g][db][4 * e + 2], x[g][db][4 * e + 3]};
-                    }
-            wg_barrier();
-            if (rg == 0) {
-#pragma unroll
-                for (int g = 0; g < KG; ++g)
-#pragma unroll
-                    for (int db = 0; db < DB; ++db)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const f32x4 v = *(reinterpret_cast<const f32x4*>(ex) + ((g * DB + db) * 4 + e) * 64 + lane);
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) x[g][db][4 * e + j] += v[j];
-                        }
-            }
-        }
-        if (rg == 1) return;
-    }
-#pragma unroll
-    for (int g = 0; g < KG; ++g) {
-        const int key = k0 + 32 * g + r;
-        if (key >= a.M) continue;
-        const long long orow = ((long long)b * a.M + key) * a.Hk + hk;
-        if (a.splits > 1) {
-            const long long rows = (long long)a.B * a.M * a.Hk;
-            float* pk = a.part + (split * rows + orow) * a.D;
-            float* pv = pk + (long long)a.splits * rows * a.D;
-#pragma unroll
-            for (int db = 0; db < DB; ++db) {
-                att_store_block_f32(pk, 32 * db, h, a.D, dk[g][db]);
-                att_store_block_f32(pv, 32 * db, h, a.D, dv[g][db]);
-            }
-            continue;
-        }
-        T* ok = (T*)a.dk + orow * a.D;
-        T* ov = (T*)a.dv + orow * a.D;
+    AttArgsMem& m = *att_args();
+    if (key >= m.M) return;
+    const long long orow = ((long long)b * m.M + key) * m.Hk + hk;
+    if (m.k_splits > 1) {
+        const long long rows = (long long)m.B * m.M * m.Hk;
+        float* pk = m.k_part + (split * rows + orow) * m.D;
+        float* pv = pk + (long long)m.k_splits * rows * m.D;
 #pragma unroll
         for (int db = 0; db < DB; ++db) {
-            att_store_block<T>(ok, 32 * db, h, a.D, dk[g][db], a.scale);
-            att_store_block<T>(ov, 32 * db, h, a.D, dv[g][db], 1.f);
+            att_store_block_f32(pk, 32 * db, h, m.D, dk[db]);
+            att_store_block_f32(pv, 32 * db, h, m.D, dv[db]);
         }
+        return;
     }
+    T* ok = (T*)m.dk + orow * m.D;
+    T* ov = (T*)m.dv + orow * m.D;
+#pragma unroll
+    for (int db = 0; db < DB; ++db) {
+        att_store_block<T>(ok, 32 * db, h, m.D, dk[db], m.scale);
+        att_store_block<T>(ov, 32 * db, h, m.D, dv[db], 1.f);
+    }
+}
+
+// one launch for both: they are independent, the workgroups of dQ fill what those of dK, dV leave idle
+template <typename T, int DP>
+__global__ __launch_bounds__(256, 2) void att_bwd_kernel(AttArgs a) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const int n = a.B * a.Hk * a.k_tiles * a.k_splits;
+    if ((int)blockIdx.x < n) att_dkdv<T, DP>(a, blockIdx.x, smem);
+    else att_dq<T, DP>(a, blockIdx.x - n, smem);
 }
 
 // out = f * sum over splits, four values per thread, splits in order (count % 4 == 0: D % 8 == 0)
@@ -446,7 +411,7 @@ int attention_check(const void* const* ptrs, int np, const long long* const* str
 
 struct AttBwdPlan {
     int q_tiles, q_splits, k_tiles, k_splits, rows_pad;
-    size_t stat_bytes, part_bytes;
+    size_t stat_bytes, q_part_bytes, k_part_bytes;
 };
 
 static AttBwdPlan attention_bwd_plan(int B, int N, int M, int H, int Hk, int D) {
@@ -476,49 +441,35 @@ static AttBwdPlan attention_bwd_plan(int B, int N, int M, int H, int Hk, int D) 
         }
     }
     p.stat_bytes = (size_t)pairs * p.rows_pad * 4 * sizeof(float);
-    const size_t a = p.q_splits > 1 ? (size_t)p.q_splits * B * N * H * D * sizeof(float) : 0;
-    const size_t c = p.k_splits > 1 ? (size_t)p.k_splits * B * M * Hk * D * 2 * sizeof(float) : 0;
-    p.part_bytes = a > c ? a : c;                                  // one after the other on one stream: shared
+    p.q_part_bytes = p.q_splits > 1 ? (size_t)p.q_splits * B * N * H * D * sizeof(float) : 0;
+    p.k_part_bytes = p.k_splits > 1 ? (size_t)p.k_splits * B * M * Hk * D * 2 * sizeof(float) : 0;
     return p;
 }
 
 template <typename T, int DP>
-static int attention_bwd_launch(AttArgs a, const AttBwdPlan& p, hipStream_t stream) {
-    static SvpsLdsAttr attr_q, attr_k;
-    constexpr int KT = 64, KG = 1, RG = KG, LDS_Q = 4 * KT * DP * 2, LDS_K = 2 * (2 * 64 * DP * 2 + 512);
-    hipError_t e = attr_q.ensure((const void*)att_dq_kernel<T, DP, KT>, LDS_Q);
-    if (e == hipSuccess) e = attr_k.ensure((const void*)att_dkdv_kernel<T, DP, KG, RG>, LDS_K);
+static int attention_bwd_launch(const AttArgs& a, const AttBwdPlan& p, hipStream_t stream) {
+    static SvpsLdsAttr attr;
+    constexpr int LDS = 2 * (2 * 64 * DP * 2 + 512) + (DP == 128 ? 8192 : 0);     // two pairs of 64-row tiles; for dK and dV their (lse, delta) and kept fragments
+    hipError_t e = attr.ensure((const void*)att_bwd_kernel<T, DP>, LDS);
     if (e != hipSuccess) return (int)e;
-    const long long pairs = (long long)a.B * a.Hk;
-    const long long lanes = pairs * a.rows_pad * (DP / 8);
+    const long long pairs = (long long)a.B * a.Hk, lanes = pairs * a.rows_pad * (DP / 8);
     hipLaunchKernelGGL((att_stats_kernel<T, DP>), dim3((unsigned)((lanes + 255) / 256)), dim3(256), 0, stream, a);
     e = hipGetLastError();
     if (e != hipSuccess) return (int)e;
-    AttArgs k = a;
-    k.tiles = p.k_tiles;
-    k.splits = p.k_splits;
-    hipLaunchKernelGGL((att_dkdv_kernel<T, DP, KG, RG>), dim3((unsigned)(pairs * k.tiles * k.splits)), dim3(256), LDS_K, stream, k);
+    const unsigned grid = (unsigned)(pairs * ((long long)a.k_tiles * a.k_splits + (long long)a.tiles * a.splits));
+    hipLaunchKernelGGL((att_bwd_kernel<T, DP>), dim3(grid), dim3(256), LDS, stream, a);
     e = hipGetLastError();
-    if (e != hipSuccess) return (int)e;
-    if (k.splits > 1) {
+    auto add = [&](const float* part, void* out, long long count, int splits, float f) {
+        if (e != hipSuccess) return;
+        hipLaunchKernelGGL(att_add_kernel<T>, dim3((unsigned)((count / 4 + 255) / 256)), dim3(256), 0, stream, part, (T*)out, count, splits, f);
+        e = hipGetLastError();
+    };
+    if (a.k_splits > 1) {
         const long long count = (long long)a.B * a.M * a.Hk * a.D;
-        const unsigned grid = (unsigned)((count / 4 + 255) / 256);
-        hipLaunchKernelGGL(att_add_kernel<T>, dim3(grid), dim3(256), 0, stream, a.part, (T*)a.dk, count, k.splits, a.scale);
-        hipLaunchKernelGGL(att_add_kernel<T>, dim3(grid), dim3(256), 0, stream, a.part + k.splits * count, (T*)a.dv, count, k.splits, 1.f);
-        e = hipGetLastError();
-        if (e != hipSuccess) return (int)e;
+        add(a.k_part, a.dk, count, a.k_splits, a.scale);
+        add(a.k_part + a.k_splits * count, a.dv, count, a.k_splits, 1.f);
     }
-    AttArgs q = a;
-    q.tiles = p.q_tiles;
-    q.splits = p.q_splits;
-    hipLaunchKernelGGL((att_dq_kernel<T, DP, KT>), dim3((unsigned)(pairs * q.tiles * q.splits)), dim3(256), LDS_Q, stream, q);
-    e = hipGetLastError();
-    if (e != hipSuccess) return (int)e;
-    if (q.splits > 1) {
-        const long long count = (long long)a.B * a.N * a.H * a.D;
-        hipLaunchKernelGGL(att_add_kernel<T>, dim3((unsigned)((count / 4 + 255) / 256)), dim3(256), 0, stream, a.part, (T*)a.dq, count, q.splits, a.scale);
-        e = hipGetLastError();
-    }
+    if (a.splits > 1) add(a.part, a.dq, (long long)a.B * a.N * a.H * a.D, a.splits, a.scale);
     return (int)e;
 }
 
@@ -527,7 +478,7 @@ static int attention_bwd_launch(AttArgs a, const AttBwdPlan& p, hipStream_t stre
 extern "C" size_t svps_attention_bwd_workspace_bytes(int B, int N, int M, int H, int Hk, int D) {
     if (B <= 0 || N <= 0 || M <= 0 || H <= 0 || Hk <= 0 || H % Hk || D <= 0) return 0;
     const svps::AttBwdPlan p = svps::attention_bwd_plan(B, N, M, H, Hk, D);
-    return p.stat_bytes + p.part_bytes;
+    return p.stat_bytes + p.q_part_bytes + p.k_part_bytes;
 }
 
 extern "C" int svps_attention_bwd(const void* dout, const long long* sd, const void* q, const long long* sq, const void* k, const long long* sk,
@@ -541,7 +492,7 @@ extern "C" int svps_attention_bwd(const void* dout, const long long* sd, const v
     const int rc = attention_check(ptrs, 9, st, 4, B, N, M, H, Hk, D, frame, window, scale, dtype);
     if (rc) return rc;
     const AttBwdPlan p = attention_bwd_plan(B, N, M, H, Hk, D);
-    if (workspace_bytes < p.stat_bytes + p.part_bytes) return SVPS_ERR_WORKSPACE;
+    if (workspace_bytes < p.stat_bytes + p.q_part_bytes + p.k_part_bytes) return SVPS_ERR_WORKSPACE;
     AttArgs a = {};
     a.q = q; a.k = k; a.v = v; a.dout = dout; a.out_in = out; a.lse = const_cast<float*>(lse);
     a.dq = dq; a.dk = dk; a.dv = dv; a.qlens = qlens; a.klens = klens;
@@ -553,7 +504,9 @@ extern "C" int svps_attention_bwd(const void* dout, const long long* sd, const v
     a.stat_lo = (int*)(a.stat_delta + rows);
     a.stat_hi = a.stat_lo + rows;
     a.part = (float*)((char*)workspace + p.stat_bytes);
+    a.k_part = (float*)((char*)workspace + p.stat_bytes + p.q_part_bytes);
     a.rows_pad = p.rows_pad;
+    a.tiles = p.q_tiles; a.splits = p.q_splits; a.k_tiles = p.k_tiles; a.k_splits = p.k_splits;
     a.B = B; a.N = N; a.M = M; a.H = H; a.Hk = Hk; a.G = H / Hk; a.D = D; a.frame = frame; a.window = window;
     a.scale = scale;
     a.gmagic = a.G > 1 ? (unsigned)(0x100000000ULL / a.G) + 1 : 0;

@@ -80,13 +80,14 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void attention_fwd_kernel
         }
     }
 
-    AttTile<DP, KT, NW> tk, tv;
-    tk.init((const T*)a.k + b * a.skb + hk * a.skh, a.skn, 0, a, 1, w, lane);
-    tv.init((const T*)a.v + b * a.svb + hk * a.svh, a.svn, 0, a, 1, w, lane);
+    AttTile<DP, KT, NW, kAttK> tk;
+    AttTile<DP, KT, NW, kAttV> tv;
+    tk.init((const T*)a.k + b * a.skb + hk * a.skh, a, w, lane);
+    tv.init((const T*)a.v + b * a.svb + hk * a.svh, a, w, lane);
     auto stage = [&](int tile, int buf) __attribute__((always_inline)) {
         char* lk = smem + buf * 2 * TILE;
-        tk.stage(a, 1, tile, klen, lk, w, lane);
-        tv.stage(a, 1, tile, klen, lk + TILE, w, lane);
+        tk.stage(tile, klen, lk, w, lane);
+        tv.stage(tile, klen, lk + TILE, w, lane);
     };
 
     f32x16 acc[DB];

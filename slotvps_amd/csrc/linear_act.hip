@@ -68,7 +68,7 @@ struct LinTile {
             for (int i = 0; i < N; ++i) {
                 const int lr = (i * NW + w) * RPP + lane / CH;
                 const int k = s * 64 + (KM ? lr : 8 * ((lane % CH) ^ lin_swz<BYTES>(lr)));
-                dma16(k < K ? b + off[i] : reinterpret_cast<const char*>(g_att_zero), lds + (i * NW + w) * 1024);
+                dma_ptr(k < K ? b + off[i] : reinterpret_cast<const char*>(g_att_zero), lds + (i * NW + w) * 1024);
             }
         }
     }
