@@ -84,7 +84,8 @@ __device__ __forceinline__ int floor_div(int x, int d) {
 }
 
 // visible keys [lo, hi) of token n (0 <= n < qlen)
-__device__ __forceinline__ void att_range(const AttArgs& a, int n, int qlen, int klen, int& lo, int& hi) {
+template <typename A>
+__device__ __forceinline__ void att_range(const A& a, int n, int qlen, int klen, int& lo, int& hi) {
     lo = 0;
     hi = klen;
     if (a.frame > 0) {
@@ -142,18 +143,23 @@ template <> struct AttVec<_Float16> { typedef f16x8 v8; typedef f16x4 v4; };
 // base moves (no address arithmetic in the loop); rows behind the last valid one and padded channels take zeros on a slower path - what
 // stands behind a length must not reach a product, 0 * NaN included.
 enum { kAttQ, kAttK, kAttV, kAttDout };
-template <int DP, int ROWS, int NW, int OP>
+template <int DP, int ROWS, int NW, int OP, bool HOLD = true>
 struct AttTile {
     static constexpr int CH = DP / 8, RPP = 64 / CH, PIECES = ROWS / RPP, N = PIECES / NW, LEAP = RPP * NW;
     static constexpr int NOFF = LEAP % 16 == 0 ? 1 : N;     // pieces 16 k rows apart have the same swizzle: one offset, the rest is uniform
     static_assert(PIECES % NW == 0, "every wave stages the same number of pieces");
     const char* base;
     long long step, leap;                       // bytes from tile to tile, from piece to piece
-    uint32_t off[NOFF];
+    uint32_t off[NOFF];                         // HOLD = false: computed per tile, for the kernel whose registers are full
+    static_assert(HOLD || NOFF == 1, "");
     bool quick;
     template <typename A> static __device__ __forceinline__ long long token(const A& a) { return 2 * (OP == kAttQ ? a.sqn : OP == kAttK ? a.skn : OP == kAttV ? a.svn : a.sdn); }
     template <typename A> static __device__ __forceinline__ long long head(const A& a) { return OP == kAttQ ? 2 * a.sqh : OP == kAttDout ? 2 * a.sdh : 0; }
     template <typename A> static __device__ __forceinline__ int group(const A& a) { return OP == kAttQ || OP == kAttDout ? a.G : 1; }
+    template <typename A> static __device__ __forceinline__ uint32_t offset(const A& a, int i, int w, int lane) {
+        const int row = (i * NW + w) * RPP + lane / CH, n = group(a) == 1 ? row : att_div_g(a, row);
+        return (uint32_t)n * (uint32_t)token(a) + (uint32_t)(row - n * group(a)) * (uint32_t)head(a) + (((lane % CH) ^ att_swz<DP>(row)) << 4);
+    }
     __device__ __forceinline__ void init(const void* p, const AttArgs& a, int w, int lane) {
         const long long sn = token(a), sh = head(a);
         const int G = group(a);
@@ -161,21 +167,22 @@ struct AttTile {
         step = sn * (ROWS / G);
         leap = NOFF == 1 ? sn * (LEAP / G) : 0;
         quick = a.D == DP && ROWS % G == 0 && (NOFF > 1 || LEAP % G == 0) && (unsigned long long)(step + sh * G) < 0x80000000ULL;
+        if constexpr (HOLD)
 #pragma unroll
-        for (int i = 0; i < NOFF; ++i) {
-            const int row = (i * NW + w) * RPP + lane / CH, n = G == 1 ? row : row / G;
-            off[i] = (uint32_t)(n * sn + (row - n * G) * sh) + (((lane % CH) ^ att_swz<DP>(row)) << 4);
-        }
+            for (int i = 0; i < NOFF; ++i) off[i] = offset(a, i, w, lane);
     }
     // tile number `tile` of `rows` valid packed rows
-    __device__ __forceinline__ void stage(int tile, int rows, char* lds, int w, int lane) const {
+    __device__ __forceinline__ void stage(int tile, int rows, char* lds, int w) const {
         if (quick && (tile + 1) * ROWS <= rows) {
             const char* b = base + tile * step;
+            uint32_t once = 0;
+            if constexpr (!HOLD) once = offset(*att_args(), 0, w, att_lane());
 #pragma unroll
-            for (int i = 0; i < N; ++i) dma_off(dma_base(b + i * leap), off[NOFF == 1 ? 0 : i], lds + (i * NW + w) * 1024);
+            for (int i = 0; i < N; ++i) dma_off(dma_base(b + i * leap), HOLD ? off[NOFF == 1 ? 0 : i] : once, lds + (i * NW + w) * 1024);
             return;
         }
         AttArgsMem& a = *att_args();
+        const int lane = att_lane();
 #pragma unroll 1
         for (int i = 0; i < N; ++i) {
             const int lr = (i * NW + w) * RPP + lane / CH, row = tile * ROWS + lr;

@@ -116,8 +116,8 @@ __device__ __forceinline__ void att_dq(const AttArgs& a, const int id, char* sme
     tv.init((const T*)a.v + b * a.svb + hk * a.svh, a, w, lane);
     auto stage = [&](int tile, int buf) __attribute__((always_inline)) {
         char* lk = smem + buf * 2 * TILE;
-        tk.stage(tile, klen, lk, w, lane);
-        tv.stage(tile, klen, lk + TILE, w, lane);
+        tk.stage(tile, klen, lk, w);
+        tv.stage(tile, klen, lk + TILE, w);
     };
     f32x16 acc[DB];
 #pragma unroll
@@ -248,8 +248,8 @@ __device__ __forceinline__ void att_dkdv(const AttArgs& a, const int id, char* s
     td.init((const T*)a.dout + b * a.sdb + hk * a.G * a.sdh, a, w, lane);
     auto stage = [&](int tile, int buf) __attribute__((always_inline)) {
         char* lq = smem + buf * BUF;
-        tq.stage(tile, qlen * a.G, lq, w, lane);
-        td.stage(tile, qlen * a.G, lq + TILE, w, lane);
+        tq.stage(tile, qlen * a.G, lq, w);
+        td.stage(tile, qlen * a.G, lq + TILE, w);
         if (w < 2) {                                               // 64 rows of lse2 (wave 0) and delta (wave 1); rows_pad is a multiple of 128
             const float* src = (w ? a.stat_delta : a.stat_lse2) + pbase + tile * QT;
             dma_off4(dma_base((const char*)src), att_lane() * 4, lq + 2 * TILE + 256 * w);

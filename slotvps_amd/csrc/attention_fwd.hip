@@ -9,10 +9,12 @@
 
 namespace svps {
 
-template <typename T, int DP, int NW, int KT>
-__global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void attention_fwd_kernel(AttArgs a) {
+template <typename T, int DP, int NW, int KT, int RB>
+// DP = 128: LDS admits two waves per SIMD; told so, the compiler uses their registers to read fragments ahead (4097 causal tokens: 148 -> 137 us)
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 128 || NW == 1 ? 2 : 4, DP == 128 ? 2 : 8))) void attention_fwd_kernel(AttArgs a) {
     typedef typename AttVec<T>::v8 v8;
-    constexpr int KS = DP / 16, DB = DP / 32, KB = KT / 32, TILE = KT * DP * 2;
+    constexpr int KS = DP / 16, DB = DP / 32, TILE = KT * DP * 2, ROWS = 32 * RB;
+    constexpr int KB = KT == 32 || (RB == 2 && DP == 128) ? 1 : 2;   // blocks of 32 keys whose scores are held at a time
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -24,164 +26,194 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void attention_fwd_kernel
     const int split = rest / a.tiles;
     const int b = pair / a.Hk, hk = pair - b * a.Hk;
     const int qlen = att_qlen(a, b), klen = att_klen(a, b);
+    const int row0 = (t * NW + w) * ROWS;                          // the wave's first row; a lane owns rows row0 + 32 i + r
+    const int wg0 = att_div_g(a, t * NW * ROWS);
 
-    const int row0 = (t * NW + w) * 32;                            // the wave's rows
-    const int row = row0 + r;
-    const int n = att_div_g(a, row);
-    const int head = hk * a.G + (row - n * a.G);
-    const bool have = n < qlen;
-    const long long orow = ((long long)b * a.N + n) * a.H + head;  // row of out / of the partial sums (n < N only)
-
-    const int wg0 = att_div_g(a, t * NW * 32);
-    if (wg0 >= qlen) {                                             // nothing valid in the workgroup: zeros, and leave
-        if (n < a.N && split == 0) {
-            T* o = (T*)a.out + orow * a.D;
-            for (int d = 8 * h; d < a.D; d += 16) *reinterpret_cast<u32x4*>(o + d) = u32x4{0, 0, 0, 0};
-            if (a.lse && h == 0) a.lse[((long long)b * a.H + head) * a.N + n] = -INFINITY;
-        }
-        if (a.splits > 1 && n < a.N && h == 0) {
-            float* ml = a.part + (long long)a.splits * a.B * a.N * a.H * a.D + (split * ((long long)a.B * a.N * a.H) + orow) * 2;
-            ml[0] = 0.f;
-            ml[1] = 0.f;
-        }
-        return;
-    }
-    int wg1 = att_div_g(a, t * NW * 32 + NW * 32 - 1);
-    wg1 = wg1 < qlen ? wg1 : qlen - 1;
-    int lo_wg, hi_wg, lo, hi, tmp;
-    att_range(a, wg0, qlen, klen, lo_wg, tmp);
-    att_range(a, wg1, qlen, klen, tmp, hi_wg);
-    att_range(a, have ? n : qlen - 1, qlen, klen, lo, hi);
-    // the wave's bounds: [lo_min, hi_max) is visited, [lo_max, hi_min) needs no comparison
+    v8 qf[RB][KS];
+    int tb = 0, te = 0, lo_min = 0, hi_min = 0, lo_max = 0, hi_max = 0;
     const int wn0 = att_div_g(a, row0);
-    int wn1 = att_div_g(a, row0 + 31);
-    wn1 = wn1 < qlen ? wn1 : qlen - 1;
     const bool wave_on = wn0 < qlen;
-    int lo_min, hi_min, lo_max, hi_max;
-    att_range(a, wave_on ? wn0 : qlen - 1, qlen, klen, lo_min, hi_min);
-    att_range(a, wn1, qlen, klen, lo_max, hi_max);
-
-    int tb = lo_wg / KT, te = hi_wg > lo_wg ? (hi_wg + KT - 1) / KT : lo_wg / KT;
-    if (a.splits > 1) {
-        const int per = (te - tb + a.splits - 1) / a.splits;
-        tb += split * per;
-        te = tb + per < te ? tb + per : te;
+    if (wg0 < qlen) {
+        int wg1 = att_div_g(a, t * NW * ROWS + NW * ROWS - 1);
+        wg1 = wg1 < qlen ? wg1 : qlen - 1;
+        int lo_wg, hi_wg, tmp;
+        att_range(a, wg0, qlen, klen, lo_wg, tmp);
+        att_range(a, wg1, qlen, klen, tmp, hi_wg);
+        // the wave's bounds: [lo_min, hi_max) is visited, [lo_max, hi_min) needs no comparison
+        int wn1 = att_div_g(a, row0 + ROWS - 1);
+        wn1 = wn1 < qlen ? wn1 : qlen - 1;
+        att_range(a, wave_on ? wn0 : qlen - 1, qlen, klen, lo_min, hi_min);
+        att_range(a, wn1, qlen, klen, lo_max, hi_max);
+        tb = lo_wg / KT;
+        te = hi_wg > lo_wg ? (hi_wg + KT - 1) / KT : tb;
+        if (a.splits > 1) {
+            const int per = (te - tb + a.splits - 1) / a.splits;
+            tb += split * per;
+            te = tb + per < te ? tb + per : te;
+        }
     }
-
-    v8 qf[KS];
-    {
+#pragma unroll
+    for (int i = 0; i < RB; ++i) {
+        const int row = row0 + 32 * i + r, n = att_div_g(a, row), head = hk * a.G + (row - n * a.G);
+        const bool have = n < qlen;
         const T* qp = (const T*)a.q + b * a.sqb + n * a.sqn + head * a.sqh;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
             const int d = 16 * ks + 8 * h;
             u32x4 x = {0, 0, 0, 0};
             if (have && d < a.D) x = *reinterpret_cast<const u32x4*>(qp + d);
-            qf[ks] = __builtin_bit_cast(v8, x);
+            qf[i][ks] = __builtin_bit_cast(v8, x);
         }
     }
 
-    AttTile<DP, KT, NW, kAttK> tk;
-    AttTile<DP, KT, NW, kAttV> tv;
+    constexpr bool HOLD = RB == 1;
+    AttTile<DP, KT, NW, kAttK, HOLD> tk;
+    AttTile<DP, KT, NW, kAttV, HOLD> tv;
     tk.init((const T*)a.k + b * a.skb + hk * a.skh, a, w, lane);
     tv.init((const T*)a.v + b * a.svb + hk * a.svh, a, w, lane);
-    auto stage = [&](int tile, int buf) __attribute__((always_inline)) {
-        char* lk = smem + buf * 2 * TILE;
-        tk.stage(tile, klen, lk, w, lane);
-        tv.stage(tile, klen, lk + TILE, w, lane);
-    };
-
-    f32x16 acc[DB];
+    f32x16 acc[RB][DB];
+    float mc[RB], l[RB];                                           // reference point of the exponentials (base 2) and their sum (this lane half's keys)
 #pragma unroll
-    for (int db = 0; db < DB; ++db)
+    for (int i = 0; i < RB; ++i) {
+        mc[i] = kAttFloor;
+        l[i] = 0.f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) acc[db][i] = 0.f;
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][db][e] = 0.f;
+    }
     const float c = a.scale * kLog2e;
     AttLane<DP> at(lane);
-    float mc = kAttFloor, l = 0.f;                                 // reference point of the exponentials (base 2) and their sum (this lane half's keys)
 
+    auto stage = [&](int tile, int buf) __attribute__((always_inline)) {
+        char* lk = smem + buf * 2 * TILE;
+        tk.stage(tile, klen, lk, w);
+        tv.stage(tile, klen, lk + TILE, w);
+    };
     if (tb < te) stage(tb, 0);
     for (int tile = tb; tile < te; ++tile) {
         const int buf = (tile - tb) & 1;
         wait_vm<0>();
         wg_barrier();                                              // the tile is here; nobody reads the other buffer any more
         if (tile + 1 < te) stage(tile + 1, buf ^ 1);
-        const int k0 = tile * KT;
-        if (!wave_on || k0 >= hi_max || k0 + KT <= lo_min) continue;
         const char* lk = smem + buf * 2 * TILE;
         const char* lv = lk + TILE;
-        at.pin();
-        float p[KB * 16];
-        float mt = -INFINITY;
-        const bool whole = k0 >= lo_max && k0 + KT <= hi_min;
+#pragma unroll 1
+        for (int sub = 0; sub < KT / (32 * KB); ++sub) {
+            const int k0 = tile * KT + 32 * KB * sub, r0 = 32 * KB * sub;
+            if (!wave_on || k0 >= hi_max || k0 + 32 * KB <= lo_min) continue;
+            at.pin();
+            f32x16 s[RB][KB];
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb) {
-            f32x16 s;
+            for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] = 0.f;
+                for (int ks = 0; ks < KS; ++ks) {
+                    const v8 kx = att_row_frag<T, DP>(lk, at, r0 + 32 * kb, ks);
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) s = mfma16(att_row_frag<T, DP>(lk, at, 32 * kb, ks), qf[ks], s);
+                    for (int i = 0; i < RB; ++i) {
+                        if (ks == 0)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) p[16 * kb + i] = s[i];
-        }
-        if (!whole) {
-            asm volatile("");                                      // a branch, not 32 selects in every tile
+                            for (int e = 0; e < 16; ++e) s[i][kb][e] = 0.f;
+                        s[i][kb] = mfma16(kx, qf[i][ks], s[i][kb]);
+                    }
+                }
+            if (!(k0 >= lo_max && k0 + 32 * KB <= hi_min)) {
+                // the rows' intervals are computed here, in the few tiles that straddle one, and hold no registers in the others
+                AttArgsMem& m = *att_args();
+                const int ln = att_lane();
 #pragma unroll
-            for (int i = 0; i < KB * 16; ++i) {
-                const int key = k0 + 32 * (i >> 4) + acc_row(i & 15, h);
-                if (key < lo || key >= hi) p[i] = -INFINITY;
+                for (int i = 0; i < RB; ++i) {
+                    const int n = att_div_g(m, row0 + 32 * i + (ln & 31));
+                    int lo, hi;
+                    att_range(m, n < qlen ? n : qlen - 1, qlen, klen, lo, hi);
+#pragma unroll
+                    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const int key = k0 + 32 * kb + acc_row(e, ln >> 5);
+                            if (key < lo || key >= hi) s[i][kb][e] = -INFINITY;
+                        }
+                }
             }
-        }
+            // The reference point of the exponentials moves only when a row's maximum has outgrown it by a factor of 2^8: until then the
+            // sums stay within 2^8 of their scale, and the rescaling (every accumulator of the wave) is skipped.
+            float mt[RB];
+            bool grown = false;
 #pragma unroll
-        for (int i = 0; i < KB * 16; ++i) mt = fmaxf(mt, p[i]);
-        // The reference point of the exponentials moves only when a row's maximum has outgrown it by a factor of 2^8: until then the sums
-        // stay within 2^8 of their scale, and the rescaling (every accumulator of the wave) is skipped.
-        if (__any(mt * c > mc + 8.f)) {
-            const float mn = fmaxf(mc, wave_half_xor_max(mt) * c);     // a row's keys are in both lane halves: one point for both
-            const float alpha = __builtin_amdgcn_exp2f(mc - mn);
-            mc = mn;
-            l *= alpha;
+            for (int i = 0; i < RB; ++i) {
+                mt[i] = -INFINITY;
 #pragma unroll
-            for (int db = 0; db < DB; ++db)
+                for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) acc[db][i] *= alpha;
-        }
+                    for (int e = 0; e < 16; ++e) mt[i] = fmaxf(mt[i], s[i][kb][e]);
+                grown = grown || mt[i] * c > mc[i] + 8.f;
+            }
+            if (__any(grown)) {
 #pragma unroll
-        for (int i = 0; i < KB * 16; ++i) {
-            p[i] = __builtin_amdgcn_exp2f(fmaf(p[i], c, -mc));
-            l += p[i];                                             // before its rounding: the backward pass divides by this sum
-        }
+                for (int i = 0; i < RB; ++i) {
+                    const float mn = fmaxf(mc[i], wave_half_xor_max(mt[i]) * c);   // a row's keys are in both lane halves: one point for both
+                    const float alpha = __builtin_amdgcn_exp2f(mc[i] - mn);
+                    mc[i] = mn;
+                    l[i] *= alpha;
 #pragma unroll
-        for (int ks = 0; ks < KT / 16; ++ks) {
-            const v8 pf = att_pack<T>(p + 8 * ks);
+                    for (int db = 0; db < DB; ++db)
 #pragma unroll
-            for (int db = 0; db < DB; ++db) acc[db] = mfma16(att_col_frag<T, DP>(lv, at, 16 * ks, db), pf, acc[db]);
+                        for (int e = 0; e < 16; ++e) acc[i][db][e] *= alpha;
+                }
+            }
+            float p[RB][KB * 16];
+#pragma unroll
+            for (int i = 0; i < RB; ++i)
+#pragma unroll
+                for (int e = 0; e < KB * 16; ++e) {
+                    p[i][e] = __builtin_amdgcn_exp2f(fmaf(s[i][e >> 4][e & 15], c, -mc[i]));
+                    l[i] += p[i][e];                               // before its rounding: the backward pass divides by this sum
+                }
+#pragma unroll
+            for (int ks = 0; ks < 2 * KB; ++ks) {
+                v8 pf[RB];
+#pragma unroll
+                for (int i = 0; i < RB; ++i) pf[i] = att_pack<T>(p[i] + 8 * ks);
+#pragma unroll
+                for (int db = 0; db < DB; ++db) {
+                    const v8 vx = att_col_frag<T, DP>(lv, at, r0 + 16 * ks, db);
+#pragma unroll
+                    for (int i = 0; i < RB; ++i) acc[i][db] = mfma16(vx, pf[i], acc[i][db]);
+                }
+            }
         }
     }
 
-    l = wave_half_xor_sum(l);
-    if (n >= a.N) return;
-    if (a.splits > 1) {
-        const long long rows = (long long)a.B * a.N * a.H;
-        float* po = a.part + (split * rows + orow) * a.D;
+    AttArgsMem& m = *att_args();
 #pragma unroll
-        for (int db = 0; db < DB; ++db) att_store_block_f32(po, 32 * db, h, a.D, acc[db]);
-        if (h == 0) {
-            float* ml = a.part + (long long)a.splits * rows * a.D + (split * rows + orow) * 2;
-            ml[0] = mc;
-            ml[1] = have ? l : 0.f;
+    for (int i = 0; i < RB; ++i) {
+        const int row = row0 + 32 * i + r, n = att_div_g(m, row), head = hk * m.G + (row - n * m.G);
+        if (n >= m.N) continue;
+        const long long orow = ((long long)b * m.N + n) * m.H + head;
+        const float sum = wave_half_xor_sum(l[i]);
+        const bool some = n < qlen && sum > 0.f;
+        if (m.splits > 1) {
+            const long long rows = (long long)m.B * m.N * m.H;
+            float* po = m.part + (split * rows + orow) * m.D;
+#pragma unroll
+            for (int db = 0; db < DB; ++db) att_store_block_f32(po, 32 * db, h, m.D, acc[i][db]);
+            if (h == 0) {
+                float* ml = m.part + (long long)m.splits * rows * m.D + (split * rows + orow) * 2;
+                ml[0] = mc[i];
+                ml[1] = some ? sum : 0.f;
+            }
+            continue;
         }
-        return;
-    }
-    const bool some = have && l > 0.f;
-    T* o = (T*)a.out + orow * a.D;
-    if (some) {
-        const float inv = 1.f / l;
+        T* o = (T*)m.out + orow * m.D;
+        const float inv = some ? 1.f / sum : 0.f;
+        if (some) {
 #pragma unroll
-        for (int db = 0; db < DB; ++db) att_store_block<T>(o, 32 * db, h, a.D, acc[db], inv);
-    } else {                                                       // no visible key, or a row behind qlen
-        for (int d = 8 * h; d < a.D; d += 16) *reinterpret_cast<u32x4*>(o + d) = u32x4{0, 0, 0, 0};
+            for (int db = 0; db < DB; ++db) att_store_block<T>(o, 32 * db, h, m.D, acc[i][db], inv);
+        } else {                                                   // no visible key, or a row behind qlen
+            for (int d = 8 * h; d < m.D; d += 16) *reinterpret_cast<u32x4*>(o + d) = u32x4{0, 0, 0, 0};
+        }
+        if (m.lse && h == 0) m.lse[((long long)b * m.H + head) * m.N + n] = some ? (mc[i] + log2f(sum)) * 0.69314718055994531f : -INFINITY;
     }
-    if (a.lse && h == 0) a.lse[((long long)b * a.H + head) * a.N + n] = some ? (mc + log2f(l)) * 0.69314718055994531f : -INFINITY;
 }
 
 // joins the splits of a row: o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s. One workgroup per row: every lane of a wave holds the
@@ -239,15 +271,19 @@ __global__ __launch_bounds__(256) void attention_combine_kernel(AttArgs a) {
     }
 }
 
-struct AttPlan { int nw, kt, tiles, splits; };
+struct AttPlan { int nw, rb, kt, tiles, splits; };
 
-static AttPlan attention_plan(int B, int N, int M, int H, int Hk) {
-    const long long rows = (long long)N * (H / Hk), pairs = (long long)B * Hk;
+// One wave of 32 rows where that is all there are. Above, four waves: of one row block each, or of two where the head size makes LDS reads
+// the bound (a fragment then serves two products; 4 x 4096 tokens, 16 heads of 128: 642 us with one, 560 us with two; of 64, where the
+// exponentials bound it, 293 and 398 us) and the workgroups are enough for four rounds. The keys are split where CUs would stand idle.
+static AttPlan attention_plan(int B, int N, int M, int H, int Hk, int D) {
+    const long long rows = (long long)N * (H / Hk), pairs = (long long)B * Hk, cus = svps_num_cus();
     AttPlan p;
     p.nw = rows <= 32 ? 1 : 4;
+    p.rb = D > 64 && pairs * ((rows + 255) / 256) >= 4 * cus ? 2 : 1;
     p.kt = p.nw == 1 ? 32 : 64;
-    p.tiles = (int)((rows + 32 * p.nw - 1) / (32 * p.nw));
-    const long long wgs = pairs * p.tiles, want = (p.nw == 1 ? 4LL : 2LL) * svps_num_cus();
+    p.tiles = (int)((rows + 32 * p.nw * p.rb - 1) / (32 * p.nw * p.rb));
+    const long long wgs = pairs * p.tiles, want = (p.nw == 1 ? 4LL : 2LL) * cus;
     const long long key_tiles = (M + p.kt - 1) / p.kt;
     long long s = wgs * 2 > want ? 1 : want / wgs;
     if (s > key_tiles / 4) s = key_tiles / 4;
@@ -256,22 +292,28 @@ static AttPlan attention_plan(int B, int N, int M, int H, int Hk) {
     return p;
 }
 
-template <typename T, int DP, int NW, int KT>
+template <typename T, int DP, int NW, int KT, int RB>
 static int attention_launch(const AttArgs& a, hipStream_t stream) {
     static SvpsLdsAttr attr;
     constexpr int LDS = 4 * KT * DP * 2;
-    const hipError_t e = attr.ensure((const void*)attention_fwd_kernel<T, DP, NW, KT>, LDS);
+    const hipError_t e = attr.ensure((const void*)attention_fwd_kernel<T, DP, NW, KT, RB>, LDS);
     if (e != hipSuccess) return (int)e;
     const unsigned grid = (unsigned)((long long)a.B * a.Hk * a.tiles * a.splits);
-    hipLaunchKernelGGL((attention_fwd_kernel<T, DP, NW, KT>), dim3(grid), dim3(64 * NW), LDS, stream, a);
+    hipLaunchKernelGGL((attention_fwd_kernel<T, DP, NW, KT, RB>), dim3(grid), dim3(64 * NW), LDS, stream, a);
     return (int)hipGetLastError();
+}
+
+template <typename T, int DP>
+static int attention_variant(const AttArgs& a, const AttPlan& p, hipStream_t stream) {
+    if (p.nw == 1) return attention_launch<T, DP, 1, 32, 1>(a, stream);
+    if constexpr (DP == 128)
+        if (p.rb == 2) return attention_launch<T, DP, 4, 64, 2>(a, stream);
+    return attention_launch<T, DP, 4, 64, 1>(a, stream);
 }
 
 template <typename T>
 static int attention_dispatch(const AttArgs& a, const AttPlan& p, hipStream_t stream) {
-    int rc;
-    if (p.nw == 1) rc = a.D <= 32 ? attention_launch<T, 32, 1, 32>(a, stream) : a.D <= 64 ? attention_launch<T, 64, 1, 32>(a, stream) : attention_launch<T, 128, 1, 32>(a, stream);
-    else rc = a.D <= 32 ? attention_launch<T, 32, 4, 64>(a, stream) : a.D <= 64 ? attention_launch<T, 64, 4, 64>(a, stream) : attention_launch<T, 128, 4, 64>(a, stream);
+    const int rc = a.D <= 32 ? attention_variant<T, 32>(a, p, stream) : a.D <= 64 ? attention_variant<T, 64>(a, p, stream) : attention_variant<T, 128>(a, p, stream);
     if (rc || a.splits == 1) return rc;
     const long long rows = (long long)a.B * a.N * a.H;
     hipLaunchKernelGGL(attention_combine_kernel<T>, dim3((unsigned)rows), dim3(256), 0, stream, a);
@@ -301,7 +343,7 @@ int attention_check(const void* const* ptrs, int np, const long long* const* str
 
 extern "C" size_t svps_attention_workspace_bytes(int B, int N, int M, int H, int Hk, int D) {
     if (B <= 0 || N <= 0 || M <= 0 || H <= 0 || Hk <= 0 || H % Hk || D <= 0) return 0;
-    const svps::AttPlan p = svps::attention_plan(B, N, M, H, Hk);
+    const svps::AttPlan p = svps::attention_plan(B, N, M, H, Hk, D);
     return p.splits > 1 ? (size_t)p.splits * B * N * H * (D + 2) * sizeof(float) : 0;
 }
 
@@ -313,7 +355,7 @@ extern "C" int svps_attention_fwd(const void* q, const long long* sq, const void
     const long long* st[] = {sq, sk, sv};
     const int rc = attention_check(ptrs, 4, st, 3, B, N, M, H, Hk, D, frame, window, scale, dtype);
     if (rc) return rc;
-    const AttPlan p = attention_plan(B, N, M, H, Hk);
+    const AttPlan p = attention_plan(B, N, M, H, Hk, D);
     const size_t need = svps_attention_workspace_bytes(B, N, M, H, Hk, D);
     if (need && (!workspace || workspace_bytes < need)) return SVPS_ERR_WORKSPACE;
     AttArgs a = {};

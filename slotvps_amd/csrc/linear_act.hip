@@ -13,6 +13,8 @@
 // holds the shared operand rows). Few tiles: the k range is split over workgroups, fp32 partial sums are added in order (same epilogue).
 //
 // Operands whose rows do not start on 16 bytes or whose length is no multiple of 8 are first copied with zero-padded rows (linear_pack).
+#include <type_traits>
+
 #include "attention.h"
 #include "../../include/slotvps_hip.h"
 
@@ -98,23 +100,21 @@ __device__ __forceinline__ typename AttVec<T>::v8 lin_frag(const char* lds, int 
 //   erfc(x) = exp(-x^2) t (a1 + t (a2 + t (a3 + t (a4 + t a5)))), t = 1 / (1 + p x), x = |z| / sqrt 2
 // with exp(-x^2) = exp(-z^2 / 2), the same exponential that the slope needs: one exponential and one reciprocal per value in place of
 // erff's two branches (measured at 32768 x 384 -> 1536: 154 us with erff, 96 us so).
-__device__ __forceinline__ void lin_act(int act, float z, float& y, float& g) {
+template <int ACT>
+__device__ __forceinline__ void lin_act(float z, float& y, float& g) {
     y = z;
     g = 1.f;
-    if (act == kActRelu) {
+    if constexpr (ACT == kActRelu) {
         y = z > 0.f ? z : z != z ? z : 0.f;
         g = z > 0.f ? 1.f : 0.f;
-    } else if (act == kActGelu) {
+    } else if constexpr (ACT == kActGelu) {
+        const float zc = fminf(fmaxf(z, -1e18f), 1e18f);           // z * z stays in range, an infinity times zero does not arise
         const float e = __builtin_amdgcn_exp2f(-0.72134752044448170f * z * z);
-        const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f * 0.70710678118654752f, fabsf(z), 1.f));
-        const float q = 0.5f * e * t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
-        const float cdf = z > 0.f ? 1.f - q : q;
-        y = z * cdf;
-        g = fmaf(z * 0.39894228040143268f, e, cdf);
-        if (!(fabsf(z) < 1e18f)) {                                 // z * z has left fp32's range: the limits, NaN stays
-            y = z > 0.f ? z : z != z ? z : 0.f;
-            g = z > 0.f ? 1.f : 0.f;
-        }
+        const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f * 0.70710678118654752f, fabsf(zc), 1.f));
+        const float q = e * t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 0.5307027145f, -0.7265760135f), 0.7107068705f), -0.142248368f), 0.127414796f);
+        const float cdf = z > 0.f ? 1.f - q : q;                   // (the half of 0.5 erfc is in the coefficients)
+        y = (z > 0.f ? z : zc) * cdf;
+        g = fmaf(zc * 0.39894228040143268f, e, cdf);
     }
 }
 
@@ -126,12 +126,12 @@ __device__ __forceinline__ float lin_bias(const LinArgs& a, int n) {
 }
 
 // N8 consecutive columns n .. of row m and their bias (8: N % 8 == 0 and 16-byte aligned tensors; 1: any)
-template <typename T, int N8>
+template <typename T, int N8, int ACT>
 __device__ __forceinline__ void lin_epilogue(const LinArgs& a, int m, int n, const float* z, const float* b) {
     const long long o = (long long)m * a.N + n;
     float y[N8], g[N8];
 #pragma unroll
-    for (int j = 0; j < N8; ++j) lin_act(a.act, z[j] + b[j], y[j], g[j]);
+    for (int j = 0; j < N8; ++j) lin_act<ACT>(z[j] + b[j], y[j], g[j]);
     if constexpr (N8 == 8) {
         if (a.residual) {
             const typename AttVec<T>::v8 r = *reinterpret_cast<const typename AttVec<T>::v8*>((const T*)a.residual + o);
@@ -151,6 +151,13 @@ __device__ __forceinline__ void lin_epilogue(const LinArgs& a, int m, int n, con
         ((T*)a.y)[o] = (T)y[0];
         if (a.gate) ((short*)a.gate)[o] = (short)(int)rintf(g[0] * kGateOne);
     }
+}
+
+template <typename T, int N8>
+__device__ __forceinline__ void lin_epilogue_any(const LinArgs& a, int m, int n, const float* z, const float* b) {
+    if (a.act == kActGelu) lin_epilogue<T, N8, kActGelu>(a, m, n, z, b);
+    else if (a.act == kActRelu) lin_epilogue<T, N8, kActRelu>(a, m, n, z, b);
+    else lin_epilogue<T, N8, kActNone>(a, m, n, z, b);
 }
 
 __device__ __forceinline__ bool lin_vec(const LinArgs& a) {
@@ -259,49 +266,55 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_kernel(LinArgs a) {
         const int n = n0 + wn * COLS + (vec ? (lane % LPR) * 8 + j : lane + 64 * j);
         bias[j] = n < a.N ? lin_bias<T>(a, n) : 0.f;
     }
+    auto store = [&](auto act) __attribute__((always_inline)) {
+        constexpr int ACT = decltype(act)::value;
 #pragma unroll
-    for (int i = 0; i < MI; ++i) {
-        const int mb = m0 + (wm * MI + i) * 32, nb = n0 + wn * COLS;
+        for (int i = 0; i < MI; ++i) {
+            const int mb = m0 + (wm * MI + i) * 32, nb = n0 + wn * COLS;
 #pragma unroll
-        for (int j = 0; j < NI; ++j)
+            for (int j = 0; j < NI; ++j)
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                f32x4 v;
+                for (int g = 0; g < 4; ++g) {
+                    f32x4 v;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * g + e];
-                *reinterpret_cast<f32x4*>(my + r * LROW + (32 * j + 8 * g + 4 * h) * 4) = v;
-            }
-        if (mb >= a.M || nb >= a.N) continue;
-        if (a.splits > 1 || vec) {
+                    for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * g + e];
+                    *reinterpret_cast<f32x4*>(my + r * LROW + (32 * j + 8 * g + 4 * h) * 4) = v;
+                }
+            if (mb >= a.M || nb >= a.N) continue;
+            if (a.splits > 1 || vec) {
 #pragma unroll
-            for (int q = 0; q < 32 / RPP; ++q) {
-                const int rr = q * RPP + lane / LPR, c = (lane % LPR) * 8, m = mb + rr, n = nb + c;
-                if (m >= a.M || n >= a.N) continue;
-                float z[8];
-                *reinterpret_cast<f32x4*>(z) = *reinterpret_cast<const f32x4*>(my + rr * LROW + c * 4);
-                *reinterpret_cast<f32x4*>(z + 4) = *reinterpret_cast<const f32x4*>(my + rr * LROW + c * 4 + 16);
-                if (a.splits > 1) {                                // ldp = N rounded up to 8
-                    float* p = a.part + ((long long)split * a.M + m) * a.ldp + n;
-                    *reinterpret_cast<f32x4*>(p) = f32x4{z[0], z[1], z[2], z[3]};
-                    *reinterpret_cast<f32x4*>(p + 4) = f32x4{z[4], z[5], z[6], z[7]};
-                } else {
-                    lin_epilogue<T, 8>(a, m, n, z, bias);
+                for (int q = 0; q < 32 / RPP; ++q) {
+                    const int rr = q * RPP + lane / LPR, c = (lane % LPR) * 8, m = mb + rr, n = nb + c;
+                    if (m >= a.M || n >= a.N) continue;
+                    float z[8];
+                    *reinterpret_cast<f32x4*>(z) = *reinterpret_cast<const f32x4*>(my + rr * LROW + c * 4);
+                    *reinterpret_cast<f32x4*>(z + 4) = *reinterpret_cast<const f32x4*>(my + rr * LROW + c * 4 + 16);
+                    if (a.splits > 1) {                            // ldp = N rounded up to 8
+                        float* p = a.part + ((long long)split * a.M + m) * a.ldp + n;
+                        *reinterpret_cast<f32x4*>(p) = f32x4{z[0], z[1], z[2], z[3]};
+                        *reinterpret_cast<f32x4*>(p + 4) = f32x4{z[4], z[5], z[6], z[7]};
+                    } else {
+                        lin_epilogue<T, 8, ACT>(a, m, n, z, bias);
+                    }
+                }
+            } else {                                               // a lane per column
+#pragma unroll
+                for (int c = 0; c < COLS / 32; c += 2) {
+                    const int cc = 32 * c + lane;
+                    if (cc >= COLS || nb + cc >= a.N) continue;
+#pragma unroll
+                    for (int rr = 0; rr < 32; ++rr)
+                        if (mb + rr < a.M) {
+                            const float z = *reinterpret_cast<const float*>(my + rr * LROW + cc * 4);
+                            lin_epilogue<T, 1, ACT>(a, mb + rr, nb + cc, &z, bias + c / 2);
+                        }
                 }
             }
-        } else {                                                   // a lane per column
-#pragma unroll
-            for (int c = 0; c < COLS / 32; c += 2) {
-                const int cc = 32 * c + lane;
-                if (cc >= COLS || nb + cc >= a.N) continue;
-#pragma unroll 4
-                for (int rr = 0; rr < 32; ++rr)
-                    if (mb + rr < a.M) {
-                        const float z = *reinterpret_cast<const float*>(my + rr * LROW + cc * 4);
-                        lin_epilogue<T, 1>(a, mb + rr, nb + cc, &z, bias + c / 2);
-                    }
-            }
         }
-    }
+    };
+    if (a.act == kActGelu) store(std::integral_constant<int, kActGelu>{});
+    else if (a.act == kActRelu) store(std::integral_constant<int, kActRelu>{});
+    else store(std::integral_constant<int, kActNone>{});
 }
 
 // the splits of a product added in order, then the same epilogue: 8 columns per thread
@@ -324,52 +337,129 @@ __global__ __launch_bounds__(256) void linear_join_kernel(LinArgs a) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) bias[j] = n + j < a.N ? lin_bias<T>(a, n + j) : 0.f;
     if (lin_vec(a)) {
-        lin_epilogue<T, 8>(a, (int)m, n, z, bias);
+        lin_epilogue_any<T, 8>(a, (int)m, n, z, bias);
     } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-            if (n + j < a.N) lin_epilogue<T, 1>(a, (int)m, n + j, z + j, bias + j);
+            if (n + j < a.N) lin_epilogue_any<T, 1>(a, (int)m, n + j, z + j, bias + j);
     }
 }
 
-// [rows, cols] with row stride ld -> [rows, ldo], ldo = cols rounded up to 8, zeros behind cols. 8 columns per thread.
-__global__ __launch_bounds__(256) void linear_pack_kernel(const uint16_t* src, long long ld, uint16_t* dst, int rows, int cols, int ldo) {
-    const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
-    const int per = ldo >> 3;
+// Few rows (M <= 16 MT): a workgroup takes 16 columns, its 8 waves every eighth 32-deep slice of k; W goes from memory to the matrix operand
+// without LDS (64 bytes of a row per lane group, each value once) with up to 4 slices of a wave in flight, the eight sums meet in LDS.
+// Bound by the read of W; one launch, no partial sums in memory.
+typedef float f32x4v __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ f32x4v mfma_16x16(bf16x8 a, bf16x8 b, f32x4v c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x4v mfma_16x16(f16x8 a, f16x8 b, f32x4v c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+
+template <typename T, int MT>
+__global__ __launch_bounds__(512) void linear_few_kernel(LinArgs a) {
+    typedef typename AttVec<T>::v8 v8;
+    __shared__ float red[8][MT][64][4];
+    const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n0 = blockIdx.x * 16;
+    const int nr = n0 + r < a.N ? n0 + r : a.N - 1;                // rows behind the end read the last one again: not stored
+    const T* wp = (const T*)a.w + nr * a.ldw + 8 * q;
+    const T* xp[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) xp[t] = (const T*)a.x + (16 * t + r < a.M ? 16 * t + r : a.M - 1) * a.ldx + 8 * q;
+    f32x4v acc[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) acc[t] = f32x4v{0.f, 0.f, 0.f, 0.f};
+    const u32x4 zero = {0, 0, 0, 0};
+    for (int k0 = 32 * w; k0 < a.K; k0 += 1024) {                  // K is a multiple of 8
+        u32x4 wv[4], xv[4][MT];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int k = k0 + 256 * u;
+            const bool in = k + 8 * q < a.K;
+            wv[u] = zero;
+            if (in) wv[u] = *reinterpret_cast<const u32x4*>(wp + k);
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                xv[u][t] = zero;
+                if (in) xv[u][t] = *reinterpret_cast<const u32x4*>(xp[t] + k);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int t = 0; t < MT; ++t) acc[t] = mfma_16x16(__builtin_bit_cast(v8, wv[u]), __builtin_bit_cast(v8, xv[u][t]), acc[t]);
+    }
+#pragma unroll
+    for (int t = 0; t < MT; ++t) *reinterpret_cast<f32x4v*>(red[w][t][lane]) = acc[t];
+    __syncthreads();
+    // lane (r, q) of a wave held row m = r and columns 4 q .. 4 q + 3 of its tile
+    for (int o = threadIdx.x; o < 256 * MT; o += 512) {
+        const int t = o >> 8, m = 16 * t + ((o >> 4) & 15), c = o & 15, n = n0 + c;
+        if (m >= a.M || n >= a.N) continue;
+        float z = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) z += red[k][t][(c >> 2) * 16 + ((o >> 4) & 15)][c & 3];
+        const float b = lin_bias<T>(a, n);
+        lin_epilogue_any<T, 1>(a, m, n, &z, &b);
+    }
+}
+
+// [rows, cols] with row stride ld -> [rows, ldo], ldo = cols rounded up to 8, zeros behind cols; two matrices in one launch (the second may
+// have no rows). 8 columns per thread.
+struct LinPack { const uint16_t* src[2]; uint16_t* dst[2]; long long ld[2]; int rows[2], cols; unsigned first; };
+
+__global__ __launch_bounds__(256) void linear_pack_kernel(LinPack a) {
+    const int which = blockIdx.x >= a.first;
+    const long long id = (long long)(blockIdx.x - (which ? a.first : 0)) * 256 + threadIdx.x;
+    const int per = (a.cols + 7) >> 3;
     const long long row = id / per;
-    if (row >= rows) return;
+    if (row >= a.rows[which]) return;
     const int c0 = (int)(id - row * per) * 8;
+    const uint16_t* src = a.src[which] + row * a.ld[which] + c0;
     union { uint16_t e[8]; u32x4 v; } o;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) o.e[j] = c0 + j < cols ? src[row * ld + c0 + j] : (uint16_t)0;
-    *reinterpret_cast<u32x4*>(dst + row * ldo + c0) = o.v;
+    for (int j = 0; j < 8; ++j) o.e[j] = c0 + j < a.cols ? src[j] : (uint16_t)0;
+    *reinterpret_cast<u32x4*>(a.dst[which] + row * (per * 8) + c0) = o.v;
 }
 
 // dz = dy * gate (stored with row stride ldz, zero padded; skipped when dz is null) and the column sums of dz over a chunk of rows.
-// Workgroup: 256 columns (32 threads x 8) x 8 rows at a time over `rows_per` rows.
+// Workgroup: 32 columns (4 threads x 8: 64 bytes of a row) x 64 rows at a time, four rows per thread in flight. One chunk: the sums are db.
 template <typename T>
-__global__ __launch_bounds__(256) void linear_dz_kernel(const T* dy, long long ldy, const short* gate, T* dz, int ldz, float* sums, int M, int N, int rows_per) {
+__global__ __launch_bounds__(256) void linear_dz_kernel(const T* dy, long long ldy, const short* gate, T* dz, int ldz, float* sums, void* db, int db_f32,
+                                                        int M, int N, int rows_per) {
     typedef typename AttVec<T>::v8 v8;
-    __shared__ float red[8][256];
-    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-    const int c0 = blockIdx.x * 256 + tx * 8;
+    typedef short s16x8 __attribute__((ext_vector_type(8)));
+    __shared__ float red[64][33];
+    const int tx = threadIdx.x & 3, ty = threadIdx.x >> 2;
+    const int c0 = blockIdx.x * 32 + tx * 8;
     const int r1 = (int)min((long long)M, ((long long)blockIdx.y + 1) * rows_per);
     const bool vec = N % 8 == 0 && !(ldy & 7) && !(((uintptr_t)dy | (uintptr_t)gate) & 15);
     float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    for (int m = blockIdx.y * rows_per + ty; m < r1; m += 8) {
-        if (c0 >= N) break;
-        float v[8];
-        if (vec) {
-            const v8 d = *reinterpret_cast<const v8*>(dy + (long long)m * ldy + c0);
+    if (c0 < N && vec) {
+        for (int mb = blockIdx.y * rows_per + ty; mb < r1; mb += 256) {
+            v8 d[4];
+            s16x8 g[4];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = (float)d[j];
-            if (gate) {
-                typedef short s16x8 __attribute__((ext_vector_type(8)));
-                const s16x8 g = *reinterpret_cast<const s16x8*>(gate + (long long)m * N + c0);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] *= (float)g[j] * (1.f / kGateOne);
+            for (int u = 0; u < 4; ++u) {
+                const long long m = mb + 64 * u < r1 ? mb + 64 * u : mb;
+                d[u] = *reinterpret_cast<const v8*>(dy + m * ldy + c0);
+                if (gate) g[u] = *reinterpret_cast<const s16x8*>(gate + m * N + c0);
             }
-        } else {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const long long m = mb + 64 * u;
+                if (m >= r1) break;
+                float v[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    v[j] = (float)d[u][j];
+                    if (gate) v[j] *= (float)g[u][j] * (1.f / kGateOne);
+                    s[j] += v[j];
+                }
+                if (dz) *reinterpret_cast<v8*>(dz + m * ldz + c0) = att_pack<T>(v);
+            }
+        }
+    } else if (c0 < N) {
+        for (int m = blockIdx.y * rows_per + ty; m < r1; m += 64) {
+            float v[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 v[j] = 0.f;
@@ -377,21 +467,23 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(const T* dy, long long l
                     v[j] = (float)dy[(long long)m * ldy + c0 + j];
                     if (gate) v[j] *= (float)gate[(long long)m * N + c0 + j] * (1.f / kGateOne);
                 }
+                s[j] += v[j];
             }
+            if (dz) *reinterpret_cast<v8*>(dz + (long long)m * ldz + c0) = att_pack<T>(v);
         }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) s[j] += v[j];
-        if (dz) *reinterpret_cast<v8*>(dz + (long long)m * ldz + c0) = att_pack<T>(v);
     }
-    if (!sums) return;
+    if (!sums && !db) return;
 #pragma unroll
     for (int j = 0; j < 8; ++j) red[ty][tx * 8 + j] = s[j];
     __syncthreads();
-    const int c = blockIdx.x * 256 + threadIdx.x;
+    const int c = blockIdx.x * 32 + threadIdx.x;
+    if (threadIdx.x >= 32 || c >= N) return;
     float t = 0.f;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) t += red[k][threadIdx.x];
-    if (c < N) sums[(long long)blockIdx.y * N + c] = t;
+#pragma unroll 16
+    for (int k = 0; k < 64; ++k) t += red[k][threadIdx.x];
+    if (sums) sums[(long long)blockIdx.y * N + c] = t;
+    else if (db_f32) ((float*)db)[c] = t;
+    else ((T*)db)[c] = (T)t;
 }
 
 // db = the chunks' sums: a workgroup takes 32 columns, eight rows of threads add every eighth chunk, the eight sums meet in LDS
@@ -417,20 +509,30 @@ __global__ __launch_bounds__(256) void linear_db_kernel(const float* sums, int c
 static inline int round8(int x) { return (x + 7) & ~7; }
 static inline bool lin_direct(const void* p, long long ld, int cols) { return !((uintptr_t)p & 15) && !(ld & 7) && !(cols & 7); }
 
-struct LinPlan { int big, splits; size_t part_bytes; };
+struct LinPlan { int tile, splits; size_t part_bytes; };
 
-// 256 x 256 tiles where they fill the chip (they read each operand value half as often from LDS), 128 x 128 otherwise; the k range is split
-// where even those leave half the chip idle.
+// Tile (256, 128 or 64 square; one, two and four workgroups of them fit a CU) and split of the k range, by a model of the time in
+// microseconds. Measured at k = 8192: a 64-deep step of a full CU takes 2.2, 0.68 and 0.36 per workgroup on it, of a workgroup alone on
+// its CU 2.2, 0.9 and 0.6; start and epilogue 6, 4 and 3; a split's partial sums go to memory and back at 4 TB/s and cost a launch.
+// (8192 cubed: 256 gives 945 us, 128 1170 us; 500 x 256 -> 2048: 128 12 us, 64 8.6 us; dW of 32768 rows, 384 -> 1536: 64 without split
+// 242 us, 128 with 14 parts 69 us.)
 static LinPlan linear_plan(int M, int N, int K) {
-    LinPlan p;
-    const int cus = svps_num_cus();
-    const long long big = ((M + 255LL) / 256) * ((N + 255LL) / 256), small = ((M + 127LL) / 128) * ((N + 127LL) / 128), want = 2LL * cus;
-    p.big = big * 4 >= cus * 3LL;
-    const long long steps = (K + 63) / 64;
-    long long s = p.big || small * 2 > want ? 1 : want / small;
-    if (s > steps / 2) s = steps / 2;
-    if (s > 64) s = 64;
-    p.splits = s < 1 ? 1 : (int)s;
+    static const int tile[3] = {256, 128, 64}, fit[3] = {1, 2, 4};
+    static const double full[3] = {2.2, 0.68, 0.36}, alone[3] = {2.2, 0.9, 0.6}, fixed[3] = {6.0, 4.0, 3.0};
+    const long long cus = svps_num_cus(), steps = (K + 63) / 64;
+    LinPlan p = {64, 1, 0};
+    double best = 0.0;
+    for (int i = 0; i < 3; ++i) {
+        const long long tiles = ((M + tile[i] - 1LL) / tile[i]) * ((N + tile[i] - 1LL) / tile[i]);
+        for (int s = 1; s <= 32 && (s == 1 || steps / s >= 4); ++s) {
+            const long long wgs = tiles * s, round = cus * fit[i], rest = wgs % round;
+            const double depth = (double)((steps + s - 1) / s);
+            auto one = [&](long long on) { const double t = on * full[i]; return depth * (t > alone[i] ? t : alone[i]) + fixed[i]; };
+            const double t = (double)(wgs / round) * one(fit[i]) + (rest ? one((rest + cus - 1) / cus) : 0.0) +
+                             (s > 1 ? 4.0 + (double)s * M * N * 8.0 / 4e6 : 0.0);
+            if (best == 0.0 || t < best) { best = t; p.tile = tile[i]; p.splits = s; }
+        }
+    }
     p.part_bytes = p.splits > 1 ? (size_t)p.splits * M * round8(N) * sizeof(float) : 0;
     return p;
 }
@@ -451,18 +553,23 @@ static int linear_launch(LinArgs a, const LinPlan& p, float* part, hipStream_t s
     a.splits = p.splits;
     a.part = part;
     a.ldp = round8(a.N);
-    const int rc = p.big ? linear_launch_tile<T, 256, 256, 2, 4, XK, WK>(a, stream) : linear_launch_tile<T, 128, 128, 2, 2, XK, WK>(a, stream);
+    const int rc = p.tile == 256 ? linear_launch_tile<T, 256, 256, 2, 4, XK, WK>(a, stream)
+                 : p.tile == 128 ? linear_launch_tile<T, 128, 128, 2, 2, XK, WK>(a, stream) : linear_launch_tile<T, 64, 64, 2, 2, XK, WK>(a, stream);
     if (rc || p.splits == 1) return rc;
     const long long threads = (long long)a.M * (a.ldp >> 3);
     hipLaunchKernelGGL(linear_join_kernel<T>, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, stream, a);
     return (int)hipGetLastError();
 }
 
-static int linear_pack(const void* src, long long ld, void* dst, int rows, int cols, hipStream_t stream) {
-    const long long threads = (long long)rows * (round8(cols) >> 3);
-    hipLaunchKernelGGL(linear_pack_kernel, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, stream, (const uint16_t*)src, ld, (uint16_t*)dst, rows, cols, round8(cols));
+static int linear_pack(const void* src, long long ld, void* dst, int rows, const void* src2, long long ld2, void* dst2, int rows2, int cols, hipStream_t stream) {
+    LinPack a = {{(const uint16_t*)src, (const uint16_t*)src2}, {(uint16_t*)dst, (uint16_t*)dst2}, {ld, ld2}, {rows, rows2}, cols, 0};
+    const long long per = (cols + 7) >> 3, g0 = (rows * per + 255) / 256, g1 = (rows2 * per + 255) / 256;
+    a.first = (unsigned)g0;
+    hipLaunchKernelGGL(linear_pack_kernel, dim3((unsigned)(g0 + g1)), dim3(256), 0, stream, a);
     return (int)hipGetLastError();
 }
+
+constexpr int kFewRows = 64;
 
 static bool linear_shape_ok(int M, int K, int N, long long ldx, long long ldw) {
     const long long big = 1LL << 30;
@@ -476,7 +583,8 @@ static bool linear_shape_ok(int M, int K, int N, long long ldx, long long ldw) {
 // workspace of a pass: aligned sections in this order
 static size_t sect(size_t bytes) { return (bytes + 255) & ~(size_t)255; }
 
-constexpr int kDzRows = 64;
+// rows per chunk of the column sums: all of them where the columns alone make enough workgroups or the rows are few, 256 otherwise
+static inline int dz_rows(int M, int N) { return M <= 512 || (N + 31) / 32 >= 4 * svps_num_cus() ? M : (M > 256 * 32768 ? (M + 32767) / 32768 : 256); }
 
 }  // namespace svps
 
@@ -484,28 +592,33 @@ extern "C" size_t svps_linear_act_workspace_bytes(int M, int K, int N, long long
     using namespace svps;
     if (!linear_shape_ok(M, K, N, ldx, ldw)) return 0;
     const bool px = unaligned || (ldx & 7) || (K & 7), pw = unaligned || (ldw & 7) || (K & 7);
-    return (px ? sect((size_t)M * round8(K) * 2) : 0) + (pw ? sect((size_t)N * round8(K) * 2) : 0) + sect(linear_plan(M, N, K).part_bytes);
+    return (px ? sect((size_t)M * round8(K) * 2) : 0) + (pw ? sect((size_t)N * round8(K) * 2) : 0) + (M <= kFewRows ? 0 : sect(linear_plan(M, N, K).part_bytes));
 }
 
 template <typename T>
 static int linear_fwd_t(svps::LinArgs a, char* ws, hipStream_t s) {
     using namespace svps;
-    const LinPlan p = linear_plan(a.M, a.N, a.K);
-    int rc;
-    if (!lin_direct(a.x, a.ldx, a.K)) {
-        if ((rc = linear_pack(a.x, a.ldx, ws, a.M, a.K, s))) return rc;
-        a.x = ws;
-        a.ldx = round8(a.K);
-        ws += sect((size_t)a.M * a.ldx * 2);
+    const bool px = !lin_direct(a.x, a.ldx, a.K), pw = !lin_direct(a.w, a.ldw, a.K);
+    const int k8 = round8(a.K);
+    if (px || pw) {
+        char* xs = ws;
+        char* wsp = ws + (px ? sect((size_t)a.M * k8 * 2) : 0);
+        const int rc = linear_pack(a.x, a.ldx, xs, px ? a.M : 0, a.w, a.ldw, wsp, pw ? a.N : 0, a.K, s);
+        if (rc) return rc;
+        if (px) { a.x = xs; a.ldx = k8; }
+        if (pw) { a.w = wsp; a.ldw = k8; }
+        ws = wsp + (pw ? sect((size_t)a.N * k8 * 2) : 0);
     }
-    if (!lin_direct(a.w, a.ldw, a.K)) {
-        if ((rc = linear_pack(a.w, a.ldw, ws, a.N, a.K, s))) return rc;
-        a.w = ws;
-        a.ldw = round8(a.K);
-        ws += sect((size_t)a.N * a.ldw * 2);
+    const int M = a.M, K = a.K;
+    a.K = k8;
+    if (M <= kFewRows) {
+        const dim3 grid((a.N + 15) / 16), block(512);
+        if (M <= 16) hipLaunchKernelGGL((linear_few_kernel<T, 1>), grid, block, 0, s, a);
+        else if (M <= 32) hipLaunchKernelGGL((linear_few_kernel<T, 2>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((linear_few_kernel<T, 4>), grid, block, 0, s, a);
+        return (int)hipGetLastError();
     }
-    a.K = round8(a.K);
-    return linear_launch<T, false, false>(a, p, (float*)ws, s);
+    return linear_launch<T, false, false>(a, linear_plan(M, a.N, K), (float*)ws, s);
 }
 
 extern "C" int svps_linear_act_fwd(const void* x, long long ldx, const void* w, long long ldw, const void* bias, int bias_f32, const void* residual,
@@ -515,7 +628,7 @@ extern "C" int svps_linear_act_fwd(const void* x, long long ldx, const void* w, 
     if (act < kActNone || act > kActGelu || (dtype != SVPS_DTYPE_BF16 && dtype != SVPS_DTYPE_F16)) return SVPS_ERR_BAD_ARG;
     if (!linear_shape_ok(M, K, N, ldx, ldw)) return SVPS_ERR_BAD_SHAPE;
     const size_t need = (lin_direct(x, ldx, K) ? 0 : sect((size_t)M * round8(K) * 2)) + (lin_direct(w, ldw, K) ? 0 : sect((size_t)N * round8(K) * 2)) +
-                        sect(linear_plan(M, N, K).part_bytes);
+                        (M <= kFewRows ? 0 : sect(linear_plan(M, N, K).part_bytes));
     if (need && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need)) return SVPS_ERR_WORKSPACE;
     LinArgs a = {};
     a.x = x; a.w = w; a.ldx = ldx; a.ldw = ldw; a.M = M; a.N = N; a.K = K;
@@ -528,11 +641,11 @@ namespace svps {
 struct LinBwdPlan { size_t dz, x, w, sums, part; int chunks; };
 static LinBwdPlan linear_bwd_plan(int M, int K, int N, bool own_dz, bool pack_x, bool pack_w, bool dx, bool dw, bool db) {
     LinBwdPlan p;
-    p.chunks = (M + kDzRows - 1) / kDzRows;
+    p.chunks = (M + dz_rows(M, N) - 1) / dz_rows(M, N);
     p.dz = own_dz ? sect((size_t)M * round8(N) * 2) : 0;
     p.x = dw && pack_x ? sect((size_t)M * round8(K) * 2) : 0;
     p.w = dx && pack_w ? sect((size_t)N * round8(K) * 2) : 0;
-    p.sums = db ? sect((size_t)p.chunks * N * sizeof(float)) : 0;
+    p.sums = db && p.chunks > 1 ? sect((size_t)p.chunks * N * sizeof(float)) : 0;
     const size_t a = dx ? linear_plan(M, K, N).part_bytes : 0, b = dw ? linear_plan(N, K, M).part_bytes : 0;
     p.part = sect(a > b ? a : b);                                  // one after the other on one stream: shared
     return p;
@@ -555,9 +668,8 @@ static int linear_bwd_t(const T* dy, long long ldy, const T* x, long long ldx, c
     char* wsp = ws; ws += p.w;
     float* sums = p.sums ? (float*)ws : nullptr; ws += p.sums;
     float* part = (float*)ws;
-    if (own || sums) {
-        // rows in chunks of kDzRows: few enough rows per workgroup to fill the chip, and the sums of a chunk are one fp32 row
-        hipLaunchKernelGGL(linear_dz_kernel<T>, dim3((N + 255) / 256, p.chunks), dim3(256), 0, s, dy, ldy, gate, own, (int)ldz, sums, M, N, kDzRows);
+    if (own || db) {
+        hipLaunchKernelGGL(linear_dz_kernel<T>, dim3((N + 31) / 32, p.chunks), dim3(256), 0, s, dy, ldy, gate, own, (int)ldz, sums, db, db_f32, M, N, dz_rows(M, N));
         hipError_t e = hipGetLastError();
         if (e != hipSuccess) return (int)e;
         if (sums) {
@@ -566,11 +678,13 @@ static int linear_bwd_t(const T* dy, long long ldy, const T* x, long long ldx, c
             if (e != hipSuccess) return (int)e;
         }
     }
+    if (p.w || p.x) {
+        if ((rc = linear_pack(x, ldx, xs, p.x ? M : 0, w, ldw, wsp, p.w ? N : 0, K, s))) return rc;
+    }
     if (dx) {                                                      // dx[m, k] = sum_n dz[m, n] W[n, k]
         LinArgs a = {};
         a.x = dz; a.ldx = ldz; a.w = w; a.ldw = ldw; a.M = M; a.N = K; a.K = N; a.y = dx;
         if (p.w) {
-            if ((rc = linear_pack(w, ldw, wsp, N, K, s))) return rc;
             a.w = wsp;
             a.ldw = round8(K);
         }
@@ -580,7 +694,6 @@ static int linear_bwd_t(const T* dy, long long ldy, const T* x, long long ldx, c
         LinArgs a = {};
         a.x = dz; a.ldx = ldz; a.w = x; a.ldw = ldx; a.M = N; a.N = K; a.K = M; a.y = dw;
         if (p.x) {
-            if ((rc = linear_pack(x, ldx, xs, M, K, s))) return rc;
             a.w = xs;
             a.ldw = round8(K);
         }
@@ -606,7 +719,6 @@ extern "C" int svps_linear_act_bwd(const void* dy, long long ldy, const void* x,
     if (!dy || (!dx && !dw && !db) || (dx && !w) || (dw && !x)) return SVPS_ERR_BAD_ARG;
     if (dtype != SVPS_DTYPE_BF16 && dtype != SVPS_DTYPE_F16) return SVPS_ERR_BAD_ARG;
     if (!linear_shape_ok(M, K, N, x ? ldx : K, w ? ldw : K) || ldy < N || ldy >= 1 << 22) return SVPS_ERR_BAD_SHAPE;
-    if ((M + kDzRows - 1) / kDzRows > 65535) return SVPS_ERR_BAD_SHAPE;
     const LinBwdPlan p = linear_bwd_plan(M, K, N, (dx || dw) && (gate || !lin_direct(dy, ldy, N)), !lin_direct(x, ldx, K), !lin_direct(w, ldw, K),
                                          dx != nullptr, dw != nullptr, db != nullptr);
     const size_t need = p.dz + p.x + p.w + p.sums + p.part;
