@@ -421,31 +421,34 @@ __global__ __launch_bounds__(256) void linear_pack_kernel(LinPack a) {
 }
 
 // dz = dy * gate (stored with row stride ldz, zero padded; skipped when dz is null) and the column sums of dz over a chunk of rows.
-// Workgroup: 32 columns (4 threads x 8: 64 bytes of a row) x 64 rows at a time, four rows per thread in flight. One chunk: the sums are db.
-template <typename T>
+// Workgroup: CT threads x 8 columns of 256 / CT rows at a time, four rows per thread in flight. CT = 32 (512 bytes of a row) for many rows;
+// CT = 4 for few, where 32-column workgroups are what fills the chip and the one chunk's sums are db (500 x 2048: 16 us wide, 7 us narrow;
+// 10240 x 1536: 7 us wide, 14 us narrow).
+template <typename T, int CT>
 __global__ __launch_bounds__(256) void linear_dz_kernel(const T* dy, long long ldy, const short* gate, T* dz, int ldz, float* sums, void* db, int db_f32,
                                                         int M, int N, int rows_per) {
     typedef typename AttVec<T>::v8 v8;
     typedef short s16x8 __attribute__((ext_vector_type(8)));
-    __shared__ float red[64][33];
-    const int tx = threadIdx.x & 3, ty = threadIdx.x >> 2;
-    const int c0 = blockIdx.x * 32 + tx * 8;
+    constexpr int RT = 256 / CT, COLS = CT * 8;
+    __shared__ float red[RT][COLS + 1];
+    const int tx = threadIdx.x % CT, ty = threadIdx.x / CT;
+    const int c0 = blockIdx.x * COLS + tx * 8;
     const int r1 = (int)min((long long)M, ((long long)blockIdx.y + 1) * rows_per);
     const bool vec = N % 8 == 0 && !(ldy & 7) && !(((uintptr_t)dy | (uintptr_t)gate) & 15);
     float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if (c0 < N && vec) {
-        for (int mb = blockIdx.y * rows_per + ty; mb < r1; mb += 256) {
+        for (int mb = blockIdx.y * rows_per + ty; mb < r1; mb += 4 * RT) {
             v8 d[4];
             s16x8 g[4];
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
-                const long long m = mb + 64 * u < r1 ? mb + 64 * u : mb;
+                const long long m = mb + RT * u < r1 ? mb + RT * u : mb;
                 d[u] = *reinterpret_cast<const v8*>(dy + m * ldy + c0);
                 if (gate) g[u] = *reinterpret_cast<const s16x8*>(gate + m * N + c0);
             }
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
-                const long long m = mb + 64 * u;
+                const long long m = mb + RT * u;
                 if (m >= r1) break;
                 float v[8];
 #pragma unroll
@@ -458,7 +461,7 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(const T* dy, long long l
             }
         }
     } else if (c0 < N) {
-        for (int m = blockIdx.y * rows_per + ty; m < r1; m += 64) {
+        for (int m = blockIdx.y * rows_per + ty; m < r1; m += RT) {
             float v[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
@@ -476,11 +479,11 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(const T* dy, long long l
 #pragma unroll
     for (int j = 0; j < 8; ++j) red[ty][tx * 8 + j] = s[j];
     __syncthreads();
-    const int c = blockIdx.x * 32 + threadIdx.x;
-    if (threadIdx.x >= 32 || c >= N) return;
+    const int c = blockIdx.x * COLS + threadIdx.x;
+    if (threadIdx.x >= COLS || c >= N) return;
     float t = 0.f;
-#pragma unroll 16
-    for (int k = 0; k < 64; ++k) t += red[k][threadIdx.x];
+#pragma unroll 8
+    for (int k = 0; k < RT; ++k) t += red[k][threadIdx.x];
     if (sums) sums[(long long)blockIdx.y * N + c] = t;
     else if (db_f32) ((float*)db)[c] = t;
     else ((T*)db)[c] = (T)t;
@@ -583,8 +586,8 @@ static bool linear_shape_ok(int M, int K, int N, long long ldx, long long ldw) {
 // workspace of a pass: aligned sections in this order
 static size_t sect(size_t bytes) { return (bytes + 255) & ~(size_t)255; }
 
-// rows per chunk of the column sums: all of them where the columns alone make enough workgroups or the rows are few, 256 otherwise
-static inline int dz_rows(int M, int N) { return M <= 512 || (N + 31) / 32 >= 4 * svps_num_cus() ? M : (M > 256 * 32768 ? (M + 32767) / 32768 : 256); }
+// rows per chunk of the column sums: all of them where they are few, 64 otherwise (at most 32768 chunks)
+static inline int dz_rows(int M) { return M <= 512 ? M : (M > 64 * 32768 ? (M + 32767) / 32768 : 64); }
 
 }  // namespace svps
 
@@ -641,7 +644,7 @@ namespace svps {
 struct LinBwdPlan { size_t dz, x, w, sums, part; int chunks; };
 static LinBwdPlan linear_bwd_plan(int M, int K, int N, bool own_dz, bool pack_x, bool pack_w, bool dx, bool dw, bool db) {
     LinBwdPlan p;
-    p.chunks = (M + dz_rows(M, N) - 1) / dz_rows(M, N);
+    p.chunks = (M + dz_rows(M) - 1) / dz_rows(M);
     p.dz = own_dz ? sect((size_t)M * round8(N) * 2) : 0;
     p.x = dw && pack_x ? sect((size_t)M * round8(K) * 2) : 0;
     p.w = dx && pack_w ? sect((size_t)N * round8(K) * 2) : 0;
@@ -669,7 +672,10 @@ static int linear_bwd_t(const T* dy, long long ldy, const T* x, long long ldx, c
     float* sums = p.sums ? (float*)ws : nullptr; ws += p.sums;
     float* part = (float*)ws;
     if (own || db) {
-        hipLaunchKernelGGL(linear_dz_kernel<T>, dim3((N + 31) / 32, p.chunks), dim3(256), 0, s, dy, ldy, gate, own, (int)ldz, sums, db, db_f32, M, N, dz_rows(M, N));
+        if (p.chunks == 1)
+            hipLaunchKernelGGL((linear_dz_kernel<T, 4>), dim3((N + 31) / 32, 1), dim3(256), 0, s, dy, ldy, gate, own, (int)ldz, sums, db, db_f32, M, N, M);
+        else
+            hipLaunchKernelGGL((linear_dz_kernel<T, 32>), dim3((N + 255) / 256, p.chunks), dim3(256), 0, s, dy, ldy, gate, own, (int)ldz, sums, db, db_f32, M, N, dz_rows(M));
         hipError_t e = hipGetLastError();
         if (e != hipSuccess) return (int)e;
         if (sums) {

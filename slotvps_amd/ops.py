@@ -1132,7 +1132,13 @@ def mask_decode_f32(feat, embed, bn_scale, bn_shift, fg_scale, fg_shift):
 
 _DTYPE_CODE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _POS_CODE = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
-_LL3 = ctypes.c_longlong * 3
+@functools.lru_cache(maxsize=4096)
+def _ll3(*strides):
+    return (ctypes.c_longlong * 3)(*strides)                     # read only by the C side
+
+
+def _at(t):
+    return None if t is None else t.data_ptr()
 
 
 def _token_tensor(t, name, dtypes):
@@ -1215,9 +1221,9 @@ def _rotary_launch(x, positions, split, base, pairing, ladder, also, inverse):
     ps = positions.stride()
     psb, psn = (0, ps[0]) if positions.dim() == 2 else (ps[0], ps[1])
     with _on(x, positions, also, y, y2) as ctx:
-        rc = lib.svps_rotary_axes(x.data_ptr(), _LL3(*x.stride()[:3]), y.data_ptr(), H,
-                                  None if also is None else also.data_ptr(), None if also is None else _LL3(*also.stride()[:3]),
-                                  None if also is None else y2.data_ptr(), 0 if also is None else also.shape[2],
+        rc = lib.svps_rotary_axes(x.data_ptr(), _ll3(*x.stride()[:3]), y.data_ptr(), H,
+                                  _at(also), None if also is None else _ll3(*also.stride()[:3]), None if also is None else y2.data_ptr(),
+                                  0 if also is None else also.shape[2],
                                   positions.data_ptr(), psb, psn, _POS_CODE[positions.dtype], len(split), csplit, turns,
                                   0 if pairing == "half" else 1, int(inverse), _DTYPE_CODE[x.dtype], B, N, D, ctx.stream)
     _lib.check(rc, "svps_rotary_axes")
@@ -1273,15 +1279,17 @@ def _att_tensor(t, name, dtype=None):
     t = _token_tensor(t, name, _TOKENS16 if dtype is None else (dtype,))
     if t.dim() != 4:
         raise ValueError(f"attention: {name} must have 4 dims [batch, tokens, heads, channels], got {tuple(t.shape)}")
-    s = t.stride()
-    if (t.data_ptr() & 15) or any((s[i] & 7) and t.shape[i] > 1 for i in range(3)):
+    a, b, c, _ = t.stride()
+    if (t.data_ptr() & 15) or ((a | b | c) & 7 and any((x & 7) and n > 1 for x, n in zip((a, b, c), t.shape))):
         t = t.clone(memory_format=torch.contiguous_format)
     return t
 
 
 def _att_strides(t):
-    s, n = t.stride(), t.shape
-    return _LL3(s[0] if n[0] > 1 else 0, s[1] if n[1] > 1 else 0, s[2] if n[2] > 1 else 0)
+    a, b, c, _ = t.stride()
+    if (a | b | c) & 7:                                          # of a dimension of one entry: never used
+        a, b, c = (x if n > 1 else 0 for x, n in zip((a, b, c), t.shape))
+    return _ll3(a, b, c)
 
 
 def _att_args(q, k, v, q_lens, k_lens, frame, window, scale):
@@ -1324,7 +1332,7 @@ def _att_fwd(q, k, v, q_lens, k_lens, frame, window, scale, want_lse):
         nbytes = _plan_bytes("svps_attention_workspace_bytes", ctx.device.index, B, N, M, H, Hk, D)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
         rc = lib.svps_attention_fwd(q.data_ptr(), _att_strides(q), k.data_ptr(), _att_strides(k), v.data_ptr(), _att_strides(v),
-                                    out.data_ptr(), _ptr(lse), _ptr(q_lens), _ptr(k_lens), _ptr(ws), nbytes, B, N, M, H, Hk, D,
+                                    out.data_ptr(), _at(lse), _at(q_lens), _at(k_lens), _at(ws), nbytes, B, N, M, H, Hk, D,
                                     frame, window, scale, _DTYPE_CODE[q.dtype], ctx.stream)
     _lib.check(rc, "svps_attention_fwd")
     return out, lse
@@ -1339,10 +1347,8 @@ def _att_bwd(dout, q, k, v, out, lse, q_lens, k_lens, frame, window, scale):
     if dout.shape != q.shape or out.shape != q.shape or lse.shape != (B, H, N):
         raise ValueError(f"attention_bwd: dout {tuple(dout.shape)}, out {tuple(out.shape)}, lse {tuple(lse.shape)} do not belong to q {tuple(q.shape)}")
     empty = B == 0 or N == 0 or M == 0
-    new = torch.zeros if empty else torch.empty
-    dq = new((B, N, H, D), dtype=q.dtype, device=q.device)
-    dk = new((B, M, Hk, D), dtype=q.dtype, device=q.device)
-    dv = new((B, M, Hk, D), dtype=q.dtype, device=q.device)
+    new = q.new_zeros if empty else q.new_empty
+    dq, dk, dv = new((B, N, H, D)), new((B, M, Hk, D)), new((B, M, Hk, D))
     if empty:
         return dq, dk, dv
     lib = _lib.load()
@@ -1351,7 +1357,7 @@ def _att_bwd(dout, q, k, v, out, lse, q_lens, k_lens, frame, window, scale):
         ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
         rc = lib.svps_attention_bwd(dout.data_ptr(), _att_strides(dout), q.data_ptr(), _att_strides(q), k.data_ptr(), _att_strides(k),
                                     v.data_ptr(), _att_strides(v), out.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-                                    _ptr(q_lens), _ptr(k_lens), ws.data_ptr(), nbytes, B, N, M, H, Hk, D, frame, window, scale,
+                                    _at(q_lens), _at(k_lens), ws.data_ptr(), nbytes, B, N, M, H, Hk, D, frame, window, scale,
                                     _DTYPE_CODE[q.dtype], ctx.stream)
     _lib.check(rc, "svps_attention_bwd")
     return dq, dk, dv
@@ -1403,8 +1409,10 @@ def attention_bwd(dout, q, k, v, out, lse, q_lens=None, k_lens=None, frame=0, wi
 def _rows16(t, name, dtype, cols):
     """[..., cols] -> 2-D rows with contiguous columns and a row stride >= cols (a view where that is possible)."""
     t = _token_tensor(t, name, (dtype,))
-    t = t.reshape(-1, cols)
-    if (cols > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and not cols <= t.stride(0) < 1 << 22):
+    if t.dim() != 2:
+        t = t.reshape(-1, cols)
+    a, b = t.stride()
+    if (cols > 1 and b != 1) or (t.shape[0] > 1 and not cols <= a < 1 << 22):
         t = t.contiguous()
     return t
 
@@ -1420,7 +1428,7 @@ def _linear_args(x, weight, bias, act, residual):
     N, K = weight.shape
     if x.shape[-1] != K or K == 0:
         raise ValueError(f"linear_act: x {tuple(x.shape)} does not match weight {tuple(weight.shape)}")
-    if max(K, N) >= 1 << 22:
+    if K >= 1 << 22 or N >= 1 << 22:
         raise ValueError("linear_act: fewer than 2^22 channels on either side")
     weight = _rows16(weight, "weight", x.dtype, K)
     if act not in (ACT_NONE, ACT_RELU, ACT_GELU):
@@ -1444,17 +1452,17 @@ def _linear_fwd(x, weight, bias, act, residual, want_gate):
     shape = x.shape[:-1] + (N,)
     y = x.new_empty(shape)
     gate = x.new_empty(shape, dtype=torch.int16) if want_gate and act != ACT_NONE else None
-    x2 = _rows16(x, "x", x.dtype, K) if x.numel() else x
-    M = y.numel() // N if N else 0
-    if M == 0:
+    if N == 0 or x.numel() == 0:
         return y, gate
+    x2 = _rows16(x, "x", x.dtype, K)
+    M = x2.shape[0]
     lib = _lib.load()
-    with _on(x, weight, bias, residual, y) as ctx:
-        ldx, ldw = _ld(x2), _ld(weight)
-        nbytes = _plan_bytes("svps_linear_act_workspace_bytes", ctx.device.index, M, K, N, ldx, ldw, (x2.data_ptr() | weight.data_ptr()) & 15)
+    with _on(x, weight, bias, residual) as ctx:
+        ldx, ldw, px, pw = _ld(x2), _ld(weight), x2.data_ptr(), weight.data_ptr()
+        nbytes = _plan_bytes("svps_linear_act_workspace_bytes", ctx.device.index, M, K, N, ldx, ldw, (px | pw) & 15)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
-        rc = lib.svps_linear_act_fwd(x2.data_ptr(), ldx, weight.data_ptr(), ldw, _ptr(bias), int(bias is not None and bias.dtype == torch.float32),
-                                     _ptr(residual), int(act), y.data_ptr(), _ptr(gate), _ptr(ws), nbytes, M, K, N, _DTYPE_CODE[x.dtype], ctx.stream)
+        rc = lib.svps_linear_act_fwd(px, ldx, pw, ldw, _at(bias), int(bias is not None and bias.dtype == torch.float32), _at(residual), act,
+                                     y.data_ptr(), _at(gate), _at(ws), nbytes, M, K, N, _DTYPE_CODE[x.dtype], ctx.stream)
     _lib.check(rc, "svps_linear_act_fwd")
     return y, gate
 
@@ -1464,10 +1472,10 @@ def _linear_bwd(dy, x, weight, gate, bias, want_dx, want_dw):
     if dy.shape != x.shape[:-1] + (N,) or (gate is not None and gate.shape != dy.shape):
         raise ValueError(f"linear_act_bwd: dy {tuple(dy.shape)} (and gate) do not belong to x {tuple(x.shape)} and weight {tuple(weight.shape)}")
     empty = dy.numel() == 0
-    new = torch.zeros if empty else torch.empty
-    dx = new(x.shape, dtype=x.dtype, device=x.device) if want_dx else None
-    dw = new((N, K), dtype=x.dtype, device=x.device) if want_dw else None
-    db = new((N,), dtype=bias.dtype, device=x.device) if bias is not None else None
+    new = x.new_zeros if empty else x.new_empty
+    dx = new(x.shape) if want_dx else None
+    dw = new((N, K)) if want_dw else None
+    db = new((N,), dtype=bias.dtype) if bias is not None else None
     if empty or not (want_dx or want_dw or bias is not None):
         return dx, dw, db
     x2, dy2 = _rows16(x, "x", x.dtype, K), _rows16(dy, "dy", x.dtype, N)
@@ -1479,8 +1487,8 @@ def _linear_bwd(dy, x, weight, gate, bias, want_dx, want_dw):
                              (x2.data_ptr() | weight.data_ptr() | dy2.data_ptr()) & 15, int(gate is not None), int(want_dx), int(want_dw),
                              int(db is not None))
         ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
-        rc = lib.svps_linear_act_bwd(dy2.data_ptr(), ldy, x2.data_ptr(), ldx, weight.data_ptr(), ldw, _ptr(gate), _ptr(dx), _ptr(dw), _ptr(db),
-                                     int(db is not None and db.dtype == torch.float32), _ptr(ws), nbytes, M, K, N, _DTYPE_CODE[x.dtype], ctx.stream)
+        rc = lib.svps_linear_act_bwd(dy2.data_ptr(), ldy, x2.data_ptr(), ldx, weight.data_ptr(), ldw, _at(gate), _at(dx), _at(dw), _at(db),
+                                     int(db is not None and db.dtype == torch.float32), _at(ws), nbytes, M, K, N, _DTYPE_CODE[x.dtype], ctx.stream)
     _lib.check(rc, "svps_linear_act_bwd")
     return dx, dw, db
 
@@ -1510,10 +1518,10 @@ def linear_act(x, weight, bias=None, act=ACT_NONE, residual=None, return_gate=Fa
     linear_act_bwd, int16 in units of 2^-14 (None for ACT_NONE).
     Differentiable in x, weight, bias, residual. fp32 tokens: slot_gemm / bgemm."""
     x, weight, residual = _linear_args(x, weight, bias, act, residual)
-    if not return_gate and torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
+    if not return_gate and torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad) or
+                                                        (residual is not None and residual.requires_grad)):
         return _LinearAct.apply(x, weight, bias, residual, act)
-    with torch.no_grad():
-        y, gate = _linear_fwd(x, weight, bias, act, residual, return_gate)
+    y, gate = _linear_fwd(x, weight, bias, act, residual, return_gate)
     return (y, gate) if return_gate else y
 
 
