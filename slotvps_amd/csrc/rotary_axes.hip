@@ -8,9 +8,10 @@
 // remainder - at most an eighth of a turn either way, exact to 2^-27 turns - goes to fp32 sine and cosine. In fp32 the product itself
 // would be off by 6e-3 radians at position 1e5.
 //
-// Bound: bandwidth (each value read once, written once; 6 operations per pair). A work item is (token, 16 bytes of a head): it computes
-// the cosines and sines of its pairs ONCE and walks over the heads of both tensors with them in registers, so the transcendental work is
-// divided by the number of heads. Few tokens: the heads are dealt over grid.y instead, one launch either way.
+// Bound: bandwidth (each value read once, written once; 6 operations per pair). A workgroup takes a few tokens: the cosines and sines of
+// their pairs once, into LDS, then all heads of both tensors as a stream of 16-byte pieces, consecutive lanes on consecutive pieces (a lane
+// per pair of pieces with the heads in a loop reads the same bytes in 96-byte shreds: 40960 tokens, 20 heads of 128: 143 us against 90 us). The
+// other half of a pair is a second read of a line that the wave has just asked for. Few tokens: the heads are dealt over grid.y.
 #include "common.h"
 #include "../../include/slotvps_hip.h"
 
@@ -27,9 +28,7 @@ struct RotArgs {
     const void* pos;                    // [B or 1, N, axes]
     long long psb, psn;                 // strides of pos (elements), last axis contiguous
     int pos_type;                       // 0 int32, 1 int64, 2 fp32
-    int B, N, D, R, items;              // items: work items per token
-    long long total;                    // B * N * items
-    int heads_per_group;
+    int B, N, D, R, tokens_per_wg, heads_per_group;
     float sign;
     double turns[kRotMaxPairs];         // f_j / (2 pi)
     unsigned char axis[kRotMaxPairs];
@@ -37,119 +36,125 @@ struct RotArgs {
 
 // the fused multiply-adds are written out: the 16-byte and the single-element form give the same bits
 template <typename T, int E> struct RotVec { typedef T type __attribute__((ext_vector_type(E))); };
+template <typename T> struct RotVec<T, 1> { typedef T type; };
 
-// E: elements per access (16 bytes, or 1). HALF: pair (j, j + R/2), otherwise (2 j, 2 j + 1).
-// items of a token: HALF: (R/2) / E rotating (two accesses each) | adjacent: R / EA rotating (one access of EA = max(E, 2)); then (D - R) / E passing
+constexpr int kRotTable = 1024;         // pairs of a workgroup's tokens
+
+// E: elements of a piece (16 bytes, or 1 where rows are not aligned or sections end inside a piece). HALF: pair (j, j + R/2), else (2 j, 2 j + 1)
 template <typename T, int E, bool HALF>
 __global__ __launch_bounds__(256) void rotary_axes_kernel(RotArgs a) {
-    constexpr int EA = HALF ? E : (E < 2 ? 2 : E);              // elements of a rotating access
-    constexpr int NP = HALF ? E : EA / 2;                       // pairs of a rotating item
+    constexpr int U = E == 1 ? 1 : 4;                            // pieces in flight
+    constexpr int NP = HALF ? E : (E + 1) / 2;                  // pairs of a piece
     typedef typename RotVec<T, E>::type VE;
-    const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (id >= a.total) return;
-    const long long tok = id / a.items;
-    const int c = (int)(id - tok * a.items);
-    const int b = (int)(tok / a.N), n = (int)(tok - (long long)b * a.N);
-    const int rot_items = HALF ? (a.R >> 1) / E : a.R / EA;
-    const int heads = a.H[0] + a.H[1];
-    const int h0 = blockIdx.y * a.heads_per_group;
-    const int h1 = h0 + a.heads_per_group < heads ? h0 + a.heads_per_group : heads;
-
-    if (c >= rot_items) {                                       // passing channels
-        const int e0 = a.R + (c - rot_items) * E;
-        for (int hh = h0; hh < h1; ++hh) {
-            const int s = hh >= a.H[0];
-            const int h = s ? hh - a.H[0] : hh;
-            const T* src = (const T*)a.x[s] + b * a.sb[s] + n * a.sn[s] + h * a.sh[s] + e0;
-            T* dst = (T*)a.y[s] + ((tok * a.H[s]) + h) * a.D + e0;
-            if constexpr (E == 1) *dst = *src;
-            else *reinterpret_cast<VE*>(dst) = *reinterpret_cast<const VE*>(src);
-        }
-        return;
-    }
-
-    const long long prow = b * a.psb + n * a.psn;
-    float cs[NP], sn[NP];
-    const int j0 = c * NP;
-#pragma unroll
-    for (int i = 0; i < NP; ++i) {
-        const int ax = a.axis[j0 + i];
+    __shared__ float2 tab[kRotTable];
+    const int pairs = a.R >> 1, tid = threadIdx.x;
+    const long long tokens = (long long)a.B * a.N, t0 = (long long)blockIdx.x * a.tokens_per_wg;
+    const int nt = (int)(tokens - t0 < a.tokens_per_wg ? tokens - t0 : a.tokens_per_wg);
+    for (int i = tid; i < nt * pairs; i += 256) {
+        const int k = i / pairs, j = i - k * pairs;
+        const long long tok = t0 + k, b = tok / a.N, at = b * a.psb + (tok - b * a.N) * a.psn + a.axis[j];
         double p;
-        if (a.pos_type == 0) p = (double)((const int*)a.pos)[prow + ax];
-        else if (a.pos_type == 1) p = (double)((const long long*)a.pos)[prow + ax];
-        else p = (double)((const float*)a.pos)[prow + ax];
-        const double t4 = 4.0 * (p * a.turns[j0 + i]);          // quarter turns
+        if (a.pos_type == 0) p = (double)((const int*)a.pos)[at];
+        else if (a.pos_type == 1) p = (double)((const long long*)a.pos)[at];
+        else p = (double)((const float*)a.pos)[at];
+        const double t4 = 4.0 * (p * a.turns[j]);               // quarter turns
         const double q = rint(t4);
         float s, co;
         sincospif(0.5f * (float)(t4 - q), &s, &co);
-        const int k = (int)(q - 4.0 * floor(0.25 * q));         // whole quarters, 0 .. 3
-        const float cc = (k & 1) ? s : co, ss = (k & 1) ? co : s;
-        cs[i] = (k == 1 || k == 2) ? -cc : cc;                  // turn by k quarters: (c, s) -> (-s, c) -> (-c, -s) -> (s, -c)
-        sn[i] = a.sign * (k >= 2 ? -ss : ss);
+        const int quarter = (int)(q - 4.0 * floor(0.25 * q));   // whole quarters, 0 .. 3
+        const float cc = (quarter & 1) ? s : co, ss = (quarter & 1) ? co : s;
+        // turn by whole quarters: (c, s) -> (-s, c) -> (-c, -s) -> (s, -c)
+        tab[i] = make_float2(quarter == 1 || quarter == 2 ? -cc : cc, a.sign * (quarter >= 2 ? -ss : ss));
     }
+    __syncthreads();
 
-    auto walk = [&](int s, int ha, int hb) {
-        const T* src = (const T*)a.x[s] + b * a.sb[s] + n * a.sn[s];
-        T* dst = (T*)a.y[s] + (tok * a.H[s]) * a.D;
-#pragma unroll 4
-        for (int h = ha; h < hb; ++h) {
-            const T* p = src + h * a.sh[s];
-            T* o = dst + (long long)h * a.D;
-            if constexpr (HALF) {
-                const int e0 = c * E, e1 = e0 + (a.R >> 1);
-                if constexpr (E == 1) {
-                    const float u = (float)p[e0], v = (float)p[e1];
-                    o[e0] = (T)fmaf(u, cs[0], -(v * sn[0]));
-                    o[e1] = (T)fmaf(v, cs[0], u * sn[0]);
-                } else {
-                    const VE u = *reinterpret_cast<const VE*>(p + e0), v = *reinterpret_cast<const VE*>(p + e1);
-                    VE yu, yv;
+    const int heads = a.H[0] + a.H[1];
+    const int h0 = blockIdx.y * a.heads_per_group;
+    const int h1 = h0 + a.heads_per_group < heads ? h0 + a.heads_per_group : heads;
+    const int per_head = a.D / E, half = a.R >> 1;
 #pragma unroll
-                    for (int i = 0; i < E; ++i) {
-                        yu[i] = (T)fmaf((float)u[i], cs[i], -((float)v[i] * sn[i]));
-                        yv[i] = (T)fmaf((float)v[i], cs[i], (float)u[i] * sn[i]);
-                    }
-                    *reinterpret_cast<VE*>(o + e0) = yu;
-                    *reinterpret_cast<VE*>(o + e1) = yv;
-                }
-            } else {
-                const int e0 = c * EA;
-                if constexpr (E == 1) {
-                    const float u = (float)p[e0], v = (float)p[e0 + 1];
-                    o[e0] = (T)fmaf(u, cs[0], -(v * sn[0]));
-                    o[e0 + 1] = (T)fmaf(v, cs[0], u * sn[0]);
-                } else {
-                    const VE x = *reinterpret_cast<const VE*>(p + e0);
-                    VE y;
+    for (int s = 0; s < 2; ++s) {
+        const int ha = s ? (h0 > a.H[0] ? h0 - a.H[0] : 0) : h0, hb = s ? h1 - a.H[0] : (h1 < a.H[0] ? h1 : a.H[0]);
+        if (ha >= hb) continue;
+        const int nh = hb - ha;
+        // piece (token k, head h, piece c) of this thread, and the step of 256 pieces as such digits
+        int c = tid % per_head, h = (tid / per_head) % nh, k = tid / per_head / nh;
+        const int dc = 256 % per_head, dh = (256 / per_head) % nh, dk = 256 / per_head / nh;
+        while (k < nt) {
+            VE own[U], other[U];
+            int pc[U], pk[U];
+            T* dst[U];
 #pragma unroll
-                    for (int i = 0; i < NP; ++i) {
-                        const float u = (float)x[2 * i], v = (float)x[2 * i + 1];
-                        y[2 * i] = (T)fmaf(u, cs[i], -(v * sn[i]));
-                        y[2 * i + 1] = (T)fmaf(v, cs[i], u * sn[i]);
-                    }
-                    *reinterpret_cast<VE*>(o + e0) = y;
+            for (int u = 0; u < U; ++u) {
+                pk[u] = k;
+                pc[u] = c;
+                if (k < nt) {
+                    const long long tok = t0 + k, b = tok / a.N;
+                    const T* src = (const T*)a.x[s] + b * a.sb[s] + (tok - b * a.N) * a.sn[s] + (long long)(ha + h) * a.sh[s];
+                    dst[u] = (T*)a.y[s] + (tok * a.H[s] + ha + h) * a.D + c * E;
+                    const int e = c * E;
+                    own[u] = *reinterpret_cast<const VE*>(src + e);
+                    if (HALF) other[u] = *reinterpret_cast<const VE*>(src + (e < half ? e + half : e < a.R ? e - half : e));
+                    else if (E == 1) other[u] = *reinterpret_cast<const VE*>(src + (e < a.R ? e ^ 1 : e));
                 }
+                c += dc;
+                h += dh;
+                k += dk;
+                if (c >= per_head) { c -= per_head; ++h; }
+                if (h >= nh) { h -= nh; ++k; }
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (pk[u] >= nt) break;
+                const int e = pc[u] * E;
+                VE y = own[u];
+                if (e < a.R) {
+                    const bool second = HALF ? e >= half : false;
+                    const float2* t = tab + pk[u] * pairs + (HALF ? (second ? e - half : e) : e >> 1);
+                    if constexpr (HALF || E == 1) {
+#pragma unroll
+                        for (int i = 0; i < E; ++i) {
+                            const float co = t[i].x, si = t[i].y;
+                            float x, z;
+                            if constexpr (E == 1) { x = (float)own[u]; z = (float)other[u]; }
+                            else { x = (float)own[u][i]; z = (float)other[u][i]; }
+                            const bool hi = HALF ? second : (e & 1);
+                            const float v = hi ? fmaf(x, co, z * si) : fmaf(x, co, -(z * si));
+                            if constexpr (E == 1) y = (T)v;
+                            else y[i] = (T)v;
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < NP; ++i) {
+                            const float u0 = (float)own[u][2 * i], v0 = (float)own[u][2 * i + 1];
+                            y[2 * i] = (T)fmaf(u0, t[i].x, -(v0 * t[i].y));
+                            y[2 * i + 1] = (T)fmaf(v0, t[i].x, u0 * t[i].y);
+                        }
+                    }
+                }
+                *reinterpret_cast<VE*>(dst[u]) = y;
             }
         }
-    };
-    const int m0 = h1 < a.H[0] ? h1 : a.H[0];
-    if (h0 < m0) walk(0, h0, m0);
-    const int k0 = h0 > a.H[0] ? h0 - a.H[0] : 0;
-    if (h1 > a.H[0]) walk(1, k0, h1 - a.H[0]);
+    }
 }
 
 template <typename T, int E, bool HALF>
 int rotary_launch(RotArgs& a, void* stream) {
-    const int rot = HALF ? (a.R >> 1) / E : a.R / (E < 2 ? 2 : E);
-    a.items = rot + (a.D - a.R) / E;
-    a.total = (long long)a.B * a.N * a.items;
-    const long long wgs = (a.total + 255) / 256;
+    const int heads = a.H[0] + a.H[1], cus = svps_num_cus();
+    const long long tokens = (long long)a.B * a.N;
+    // tokens of a workgroup: eight pieces per thread, as far as the table holds them, fewer where that leaves a CU without four workgroups;
+    // one each and still fewer: the heads are dealt out
+    long long per = kRotTable / (a.R >> 1);
+    const long long pieces = (long long)heads * (a.D / E), many = (2048 + pieces - 1) / pieces;
+    if (per > many) per = many;
+    if (per > tokens / (4 * cus)) per = tokens / (4 * cus);
+    if (per < 1) per = 1;
+    const long long wgs = (tokens + per - 1) / per;
     if (wgs > 0x7fffffffLL) return SVPS_ERR_BAD_SHAPE;
-    // enough work items for 8 waves per SIMD's worth of loads in flight (4 workgroups per CU): below that the heads are dealt out
-    const int heads = a.H[0] + a.H[1];
-    const long long want = 4LL * svps_num_cus();
-    long long groups = wgs >= want ? 1 : (want + wgs - 1) / wgs;
-    if (groups > heads) groups = heads;
+    long long groups = wgs >= 4 * cus ? 1 : (4 * cus + wgs - 1) / wgs;
+    const long long least = (256 * E + a.D - 1) / a.D;           // heads that give every thread a piece
+    if (groups > (heads + least - 1) / least) groups = (heads + least - 1) / least;
+    a.tokens_per_wg = (int)per;
     a.heads_per_group = (heads + (int)groups - 1) / (int)groups;
     const int gy = (heads + a.heads_per_group - 1) / a.heads_per_group;
     hipLaunchKernelGGL((rotary_axes_kernel<T, E, HALF>), dim3((unsigned)wgs, gy), dim3(256), 0, static_cast<hipStream_t>(stream), a);
