@@ -110,7 +110,11 @@ static __device__ __attribute__((aligned(16))) uint32_t g_att_zero[4];       // 
 // LDS-DMA: 64 lanes x 16 (4) bytes to lds_base + lane * 16 (4), with a wave-uniform base (64-bit, scalar registers) and a 32-bit lane offset
 // below 2 GiB, or with a 64-bit address per lane. Written as instructions: behind the builtin the compiler knows of a pending write to LDS
 // and waits for ALL of them in front of every transposed read, i.e. for the tile it has just asked for. Nothing is returned to a register;
-// the waits are the ones in the code (wait_vm in front of the barrier that hands a tile over).
+// the waits are the ones in the code (wait_vm in front of the barrier that hands a tile over). They are ordered against the barriers
+// (volatile) and free against LDS reads, which only touch the other buffer between two barriers. The address unit takes 16 cycles for
+// each: issued in a row behind a barrier they can hold every wave of the CU up. The forward kernel and dQ ask for the next tile behind
+// their first products (4097 causal tokens, 16 / 4 heads of 128: 110 -> 100 us forward); dK / dV and the products of linear_act ask right
+// behind the barrier (behind the products: 4097 tokens 300 -> 322 us, 8192^3 935 -> 970 us).
 __device__ __forceinline__ uint32_t lds_address(const char* p) {
     return __builtin_amdgcn_readfirstlane((uint32_t)reinterpret_cast<uintptr_t>(p));        // the low half of a flat address into LDS
 }
@@ -121,17 +125,17 @@ __device__ __forceinline__ u32x4 dma_base(const char* base) {
 __device__ __forceinline__ void dma_off(u32x4 base, uint32_t lane_off, const char* lds_base) {
     uint32_t keep;
     asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, 0 offen lds\n\ts_mov_b32 m0, %0"
-                 : "=&s"(keep) : "s"(lds_address(lds_base)), "v"(lane_off), "s"(base) : "memory");
+                 : "=&s"(keep) : "s"(lds_address(lds_base)), "v"(lane_off), "s"(base));
 }
 __device__ __forceinline__ void dma_off4(u32x4 base, uint32_t lane_off, const char* lds_base) {
     uint32_t keep;
     asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dword %2, %3, 0 offen lds\n\ts_mov_b32 m0, %0"
-                 : "=&s"(keep) : "s"(lds_address(lds_base)), "v"(lane_off), "s"(base) : "memory");
+                 : "=&s"(keep) : "s"(lds_address(lds_base)), "v"(lane_off), "s"(base));
 }
 __device__ __forceinline__ void dma_ptr(const char* src, const char* lds_base) {
     uint32_t keep;
     asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off\n\ts_mov_b32 m0, %0"
-                 : "=&s"(keep) : "s"(lds_address(lds_base)), "v"(src) : "memory");
+                 : "=&s"(keep) : "s"(lds_address(lds_base)), "v"(src));
 }
 
 template <typename T> struct AttVec;

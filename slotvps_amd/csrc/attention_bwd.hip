@@ -131,9 +131,11 @@ __device__ __forceinline__ void att_dq(const AttArgs& a, const int id, char* sme
         const int buf = (tile - tb) & 1;
         wait_vm<0>();
         wg_barrier();
-        if (tile + 1 < te) stage(tile + 1, buf ^ 1);
         const int k0 = tile * KT;
-        if (!wave_on || k0 >= hi_max || k0 + KT <= lo_min) continue;
+        if (!wave_on || k0 >= hi_max || k0 + KT <= lo_min) {
+            if (tile + 1 < te) stage(tile + 1, buf ^ 1);
+            continue;
+        }
         const char* lk = smem + buf * 2 * TILE;
         const char* lv = lk + TILE;
         at.pin();
@@ -148,6 +150,7 @@ __device__ __forceinline__ void att_dq(const AttArgs& a, const int id, char* sme
                 s = mfma16(att_row_frag<T, DP>(lk, at, 32 * kb, ks), qf[ks], s);
                 dp = mfma16(att_row_frag<T, DP>(lv, at, 32 * kb, ks), df[ks], dp);
             }
+            if (kb == 0 && tile + 1 < te) stage(tile + 1, buf ^ 1);
             float ds[16];
 #pragma unroll
             for (int i = 0; i < 16; ++i) {

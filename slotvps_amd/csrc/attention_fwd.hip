@@ -95,9 +95,9 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
         const int buf = (tile - tb) & 1;
         wait_vm<0>();
         wg_barrier();                                              // the tile is here; nobody reads the other buffer any more
-        if (tile + 1 < te) stage(tile + 1, buf ^ 1);
         const char* lk = smem + buf * 2 * TILE;
         const char* lv = lk + TILE;
+        bool asked = tile + 1 >= te;                               // the next tile: asked for behind the first products
 #pragma unroll 1
         for (int sub = 0; sub < KT / (32 * KB); ++sub) {
             const int k0 = tile * KT + 32 * KB * sub, r0 = 32 * KB * sub;
@@ -117,6 +117,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
                         s[i][kb] = mfma16(kx, qf[i][ks], s[i][kb]);
                     }
                 }
+            if (!asked) stage(tile + 1, buf ^ 1);
+            asked = true;
             if (!(k0 >= lo_max && k0 + 32 * KB <= hi_min)) {
                 // the rows' intervals are computed here, in the few tiles that straddle one, and hold no registers in the others
                 AttArgsMem& m = *att_args();
@@ -182,6 +184,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
                 }
             }
         }
+        if (!asked) stage(tile + 1, buf ^ 1);
     }
 
     AttArgsMem& m = *att_args();
