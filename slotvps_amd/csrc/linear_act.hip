@@ -197,11 +197,6 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_kernel(LinArgs a) {
     LinTile<BN, NW, WK> tw;
     tx.init(a.x, a.ldx, m0, a.M, w, lane);
     tw.init(a.w, a.ldw, n0, a.N, w, lane);
-    auto stage = [&](int s) __attribute__((always_inline)) {
-        char* l = smem + ((s - sb) & 1) * (XB + WB);
-        tx.stage(s, a.K, l, w, lane);
-        tw.stage(s, a.K, l + XB, w, lane);
-    };
     f32x16 acc[MI][NI];
 #pragma unroll
     for (int i = 0; i < MI; ++i)
@@ -209,48 +204,121 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_kernel(LinArgs a) {
         for (int j = 0; j < NI; ++j)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-    // Operand fragments one 16-deep slice ahead of the products. The barrier stands BEFORE the last slice's products: by then the step's
-    // tile is in registers, so the tile after next may overwrite it, the next one has had a step to arrive, and its first fragments are
-    // read under the last products.
     v8 xf[2][MI], wf[2][NI];
-    auto fetch = [&](int s, int ks, int to) __attribute__((always_inline)) {
-        const char* lx = smem + ((s - sb) & 1) * (XB + WB);
+    auto fetch = [&](const char* lx, const char* lw, int ks, int to) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < NI; ++j) wf[to][j] = lin_frag<T, BN, WK>(lw, (wn * NI + j) * 32, ks, lane);
 #pragma unroll
         for (int i = 0; i < MI; ++i) xf[to][i] = lin_frag<T, BM, XK>(lx, (wm * MI + i) * 32, ks, lane);
-#pragma unroll
-        for (int j = 0; j < NI; ++j) wf[to][j] = lin_frag<T, BN, WK>(lx + XB, (wn * NI + j) * 32, ks, lane);
     };
-    // the scheduling fences keep the reads in front of the products that do not need them (left alone, the compiler sinks every read to
-    // just before its use and waits for it there)
     auto multiply = [&](int from) __attribute__((always_inline)) {
-        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < MI; ++i)
 #pragma unroll
             for (int j = 0; j < NI; ++j) acc[i][j] = mfma16(wf[from][j], xf[from][i], acc[i][j]);
-        __builtin_amdgcn_sched_barrier(0);
     };
-    if (sb < se) {
-        stage(sb);
-        wait_vm<0>();
+    // (the scheduling fences keep reads, requests and products where they stand: left alone, the compiler sinks every read to just before
+    // its use and waits for it there)
+    auto fence = []() __attribute__((always_inline)) { __builtin_amdgcn_sched_barrier(0); };
+    if constexpr (NW == 8) {
+        // One workgroup per CU, two waves per SIMD that take turns: while the first four multiply half a step (16 products, 512 cycles),
+        // the others read their fragments of the next half and ask for operand tiles; then they change places, a barrier each time. A wave
+        // held up by a request or a read never holds products up (8192 cubed: 810 us; both waves doing the same, the requests behind one
+        // barrier per step, 935; the requests between a wave's own products 950).
+        // LDS holds two tiles of w and three of x (160 KB). Phases: the first waves read tile s in 4 s and 4 s + 2, the second in 4 s + 1
+        // and 4 s + 3, so its place is free from 4 s + 4 on. In step s the tiles w of s + 1 and x of s + 2 are asked for (phases 4 s, 4 s + 1
+        // and 4 s + 2, 4 s + 3); before the barrier that ends 4 s + 3 every wave waits for its pieces of both tiles of s + 1, and only its
+        // pieces of x of s + 2 stay in flight.
+        const bool second = w >= 4;
+        auto stage_x = [&](int s, int buf) __attribute__((always_inline)) { tx.stage(s, a.K, smem + buf * XB, w, lane); };
+        auto stage_w = [&](int s) __attribute__((always_inline)) { tw.stage(s, a.K, smem + 3 * XB + ((s - sb) & 1) * WB, w, lane); };
+        auto landed = [&](bool more) __attribute__((always_inline)) {
+            if (more) wait_vm<decltype(tx)::N>();
+            else wait_vm<0>();
+        };
+        if (sb < se) {
+            stage_w(sb);
+            stage_x(sb, 0);
+            if (sb + 1 < se) stage_x(sb + 1, 1);
+            landed(sb + 1 < se);
+        }
         wg_barrier();
-        if (sb + 1 < se) stage(sb + 1);
-        fetch(sb, 0, 0);
-    }
-    for (int s = sb; s < se; ++s) {
-        fetch(s, 1, 1);
-        multiply(0);
-        fetch(s, 2, 0);
-        multiply(1);
-        fetch(s, 3, 1);
-        multiply(0);
-        if (s + 1 < se) {
+        if (second) wg_barrier();                                  // a phase behind
+        int xb = 0;
+        for (int s = sb; s < se; ++s) {
+            const char* lx = smem + xb * XB;
+            const char* lw = smem + 3 * XB + ((s - sb) & 1) * WB;
+            auto half = [&](auto which) __attribute__((always_inline)) {
+                constexpr int HALF = decltype(which)::value;
+                auto ask = [&]() __attribute__((always_inline)) {
+                    if (HALF == 0) {
+                        if (s + 1 < se) stage_w(s + 1);
+                    } else {
+                        if (s + 2 < se) stage_x(s + 2, xb == 0 ? 2 : xb - 1);
+                    }
+                };
+                // reads first; where both operands are read transposed (twice the reads) the requests (dW at 8192 cubed: 900 and 850 us;
+                // the row-major product 810 and 825 us)
+                if constexpr (XK && WK) {
+                    ask();
+                    fence();
+                }
+                fetch(lx, lw, 2 * HALF, 0);
+                fetch(lx, lw, 2 * HALF + 1, 1);
+                if constexpr (!(XK && WK)) ask();
+                if (HALF == 1 && second) landed(s + 2 < se);
+                fence();
+                wg_barrier();
+                fence();
+                multiply(0);
+                multiply(1);
+                fence();
+                if (HALF == 1 && !second) landed(s + 2 < se);
+                wg_barrier();
+                fence();
+            };
+            half(std::integral_constant<int, 0>{});
+            half(std::integral_constant<int, 1>{});
+            xb = xb == 2 ? 0 : xb + 1;
+        }
+        if (!second) wg_barrier();
+    } else {
+        // Several workgroups per CU overlap by themselves. Fragments are read one 16-deep slice ahead of the products. The barrier stands
+        // BEFORE the last slice's products: by then the step's tile is in registers, so the tile after next may overwrite it, the next one
+        // has had a step to arrive, and its first fragments are read under the last products.
+        auto tile = [&](int s) __attribute__((always_inline)) { return smem + ((s - sb) & 1) * (XB + WB); };
+        auto stage = [&](int s) __attribute__((always_inline)) {
+            tx.stage(s, a.K, tile(s), w, lane);
+            tw.stage(s, a.K, tile(s) + XB, w, lane);
+        };
+        auto read = [&](int s, int ks, int to) __attribute__((always_inline)) { fetch(tile(s), tile(s) + XB, ks, to); };
+        auto products = [&](int from) __attribute__((always_inline)) {
+            fence();
+            multiply(from);
+            fence();
+        };
+        if (sb < se) {
+            stage(sb);
             wait_vm<0>();
             wg_barrier();
-            if (s + 2 < se) stage(s + 2);
-            fetch(s + 1, 0, 0);
+            if (sb + 1 < se) stage(sb + 1);
+            read(sb, 0, 0);
         }
-        multiply(1);
+        for (int s = sb; s < se; ++s) {
+            read(s, 1, 1);
+            products(0);
+            read(s, 2, 0);
+            products(1);
+            read(s, 3, 1);
+            products(0);
+            if (s + 1 < se) {
+                wait_vm<0>();
+                wg_barrier();
+                if (s + 2 < se) stage(s + 2);
+                read(s + 1, 0, 0);
+            }
+            products(1);
+        }
     }
     // Epilogue: a wave turns its 32-row blocks around through its own piece of LDS, so that 8 lanes write 128 consecutive bytes of a row
     // (straight from the accumulators a lane would hold 4 columns of its own row: 32 rows per access, four times the cache-line visits).
@@ -515,13 +583,13 @@ static inline bool lin_direct(const void* p, long long ld, int cols) { return !(
 struct LinPlan { int tile, splits; size_t part_bytes; };
 
 // Tile (256, 128 or 64 square; one, two and four workgroups of them fit a CU) and split of the k range, by a model of the time in
-// microseconds. Measured at k = 8192: a 64-deep step of a full CU takes 2.2, 0.68 and 0.36 per workgroup on it, of a workgroup alone on
-// its CU 2.2, 0.9 and 0.6; start and epilogue 6, 4 and 3; a split's partial sums go to memory and back at 4 TB/s and cost a launch.
-// (8192 cubed: 256 gives 945 us, 128 1170 us; 500 x 256 -> 2048: 128 12 us, 64 8.6 us; dW of 32768 rows, 384 -> 1536: 64 without split
+// microseconds. Measured at k = 8192: a 64-deep step of a full CU takes 1.5, 0.68 and 0.36 per workgroup on it, of a workgroup alone on
+// its CU 1.5, 0.9 and 0.6; start and epilogue 6, 4 and 3; a split's partial sums go to memory and back at 4 TB/s and cost a launch.
+// (8192 cubed: 256 gives 810 us, 128 1170 us; 500 x 256 -> 2048: 128 12 us, 64 8.6 us; dW of 32768 rows, 384 -> 1536: 64 without split
 // 242 us, 128 with 14 parts 69 us.)
 static LinPlan linear_plan(int M, int N, int K) {
     static const int tile[3] = {256, 128, 64}, fit[3] = {1, 2, 4};
-    static const double full[3] = {2.2, 0.68, 0.36}, alone[3] = {2.2, 0.9, 0.6}, fixed[3] = {6.0, 4.0, 3.0};
+    static const double full[3] = {1.5, 0.68, 0.36}, alone[3] = {1.5, 0.9, 0.6}, fixed[3] = {6.0, 4.0, 3.0};
     const long long cus = svps_num_cus(), steps = (K + 63) / 64;
     LinPlan p = {64, 1, 0};
     double best = 0.0;
@@ -542,7 +610,7 @@ static LinPlan linear_plan(int M, int N, int K) {
 
 template <typename T, int BM, int BN, int WM, int WN, bool XK, bool WK>
 static int linear_launch_tile(const LinArgs& a, hipStream_t stream) {
-    constexpr int LDS = 2 * (BM + BN) * 128;
+    constexpr int LDS = (2 * (BM + BN) + (WM * WN == 8 ? BM : 0)) * 128;
     static SvpsLdsAttr attr;
     const hipError_t e = attr.ensure((const void*)linear_kernel<T, BM, BN, WM, WN, XK, WK>, LDS);
     if (e != hipSuccess) return (int)e;
