@@ -124,20 +124,47 @@ template <typename T>
 __device__ __forceinline__ float lin_bias(const LinArgs& a, int n) {
     return !a.bias ? 0.f : a.bias_f32 ? ((const float*)a.bias)[n] : (float)((const T*)a.bias)[n];
 }
+// of columns n, n + 1, ..: all on the way before the first is used. Columns behind the end take the last one's
+template <typename T, int C>
+__device__ __forceinline__ void lin_bias(const LinArgs& a, int n, float* b) {
+#pragma unroll
+    for (int j = 0; j < C; ++j) b[j] = 0.f;
+    if (!a.bias) return;
+    if (a.bias_f32) {
+#pragma unroll
+        for (int j = 0; j < C; ++j) b[j] = ((const float*)a.bias)[n + j < a.N ? n + j : a.N - 1];
+    } else {
+        T x[C];
+#pragma unroll
+        for (int j = 0; j < C; ++j) x[j] = ((const T*)a.bias)[n + j < a.N ? n + j : a.N - 1];
+#pragma unroll
+        for (int j = 0; j < C; ++j) b[j] = (float)x[j];
+    }
+}
 
-// N8 consecutive columns n .. of row m and their bias (8: N % 8 == 0 and 16-byte aligned tensors; 1: any)
+// N8 consecutive columns n .. of row m (8: N % 8 == 0 and 16-byte aligned tensors; 1: any): their residual, asked for on its own so that a
+// caller with several rows has all of them on the way before its first store (a load after a store waits for both; 40001 x 256 -> 333:
+// 61 us row by row)
+template <typename T, int N8> struct LinRow;
+template <typename T> struct LinRow<T, 8> { typename AttVec<T>::v8 r; };
+template <typename T> struct LinRow<T, 1> { T r[1]; };
+
+template <typename T, int N8>
+__device__ __forceinline__ LinRow<T, N8> lin_residual(const LinArgs& a, int m, int n) {
+    return *reinterpret_cast<const LinRow<T, N8>*>((const T*)a.residual + (long long)m * a.N + n);
+}
+
+// and what becomes of their products z with the bias b
 template <typename T, int N8, int ACT>
-__device__ __forceinline__ void lin_epilogue(const LinArgs& a, int m, int n, const float* z, const float* b) {
+__device__ __forceinline__ void lin_epilogue(const LinArgs& a, int m, int n, const float* z, const float* b, const LinRow<T, N8>& res) {
     const long long o = (long long)m * a.N + n;
     float y[N8], g[N8];
 #pragma unroll
-    for (int j = 0; j < N8; ++j) lin_act<ACT>(z[j] + b[j], y[j], g[j]);
+    for (int j = 0; j < N8; ++j) {
+        lin_act<ACT>(z[j] + b[j], y[j], g[j]);
+        if (a.residual) y[j] += (float)res.r[j];
+    }
     if constexpr (N8 == 8) {
-        if (a.residual) {
-            const typename AttVec<T>::v8 r = *reinterpret_cast<const typename AttVec<T>::v8*>((const T*)a.residual + o);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) y[j] += (float)r[j];
-        }
         *reinterpret_cast<typename AttVec<T>::v8*>((T*)a.y + o) = att_pack<T>(y);
         if (a.gate) {
             typedef short s16x8 __attribute__((ext_vector_type(8)));
@@ -147,7 +174,6 @@ __device__ __forceinline__ void lin_epilogue(const LinArgs& a, int m, int n, con
             *reinterpret_cast<s16x8*>((short*)a.gate + o) = q;
         }
     } else {
-        if (a.residual) y[0] += (float)((const T*)a.residual)[o];
         ((T*)a.y)[o] = (T)y[0];
         if (a.gate) ((short*)a.gate)[o] = (short)(int)rintf(g[0] * kGateOne);
     }
@@ -155,9 +181,11 @@ __device__ __forceinline__ void lin_epilogue(const LinArgs& a, int m, int n, con
 
 template <typename T, int N8>
 __device__ __forceinline__ void lin_epilogue_any(const LinArgs& a, int m, int n, const float* z, const float* b) {
-    if (a.act == kActGelu) lin_epilogue<T, N8, kActGelu>(a, m, n, z, b);
-    else if (a.act == kActRelu) lin_epilogue<T, N8, kActRelu>(a, m, n, z, b);
-    else lin_epilogue<T, N8, kActNone>(a, m, n, z, b);
+    LinRow<T, N8> res = {};
+    if (a.residual) res = lin_residual<T, N8>(a, m, n);
+    if (a.act == kActGelu) lin_epilogue<T, N8, kActGelu>(a, m, n, z, b, res);
+    else if (a.act == kActRelu) lin_epilogue<T, N8, kActRelu>(a, m, n, z, b, res);
+    else lin_epilogue<T, N8, kActNone>(a, m, n, z, b, res);
 }
 
 __device__ __forceinline__ bool lin_vec(const LinArgs& a) {
@@ -328,17 +356,15 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_kernel(LinArgs a) {
     char* my = smem + w * 32 * LROW;
     const bool vec = lin_vec(a);
     constexpr int LPR = COLS / 8, RPP = 64 / LPR;                  // lanes per row, rows per pass
+    constexpr int RPL = 64 / COLS;                                 // rows per pass with a lane per column
+    static_assert(COLS == 32 || COLS == 64, "a lane per column");
     float bias[8];                                                 // a lane's columns are the same in every pass
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const int n = n0 + wn * COLS + (vec ? (lane % LPR) * 8 + j : lane + 64 * j);
-        bias[j] = n < a.N ? lin_bias<T>(a, n) : 0.f;
-    }
-    auto store = [&](auto act) __attribute__((always_inline)) {
-        constexpr int ACT = decltype(act)::value;
-#pragma unroll
-        for (int i = 0; i < MI; ++i) {
-            const int mb = m0 + (wm * MI + i) * 32, nb = n0 + wn * COLS;
+    if (a.splits == 1) lin_bias<T, 8>(a, n0 + wn * COLS + (vec ? (lane % LPR) * 8 : lane % COLS), bias);
+    auto block = [&](auto which, auto act) __attribute__((always_inline)) {
+        constexpr int i = decltype(which)::value, ACT = decltype(act)::value;
+        const int mb = m0 + (wm * MI + i) * 32, nb = n0 + wn * COLS;
+        if (mb >= a.M || nb >= a.N) return;
+        auto turn = [&]() __attribute__((always_inline)) {
 #pragma unroll
             for (int j = 0; j < NI; ++j)
 #pragma unroll
@@ -348,12 +374,22 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_kernel(LinArgs a) {
                     for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * g + e];
                     *reinterpret_cast<f32x4*>(my + r * LROW + (32 * j + 8 * g + 4 * h) * 4) = v;
                 }
-            if (mb >= a.M || nb >= a.N) continue;
-            if (a.splits > 1 || vec) {
+        };
+        if (a.splits > 1 || vec) {
+            const int c = (lane % LPR) * 8, n = nb + c;
+            LinRow<T, 8> res[32 / RPP];
+            if (a.residual && a.splits == 1 && n < a.N) {
 #pragma unroll
                 for (int q = 0; q < 32 / RPP; ++q) {
-                    const int rr = q * RPP + lane / LPR, c = (lane % LPR) * 8, m = mb + rr, n = nb + c;
-                    if (m >= a.M || n >= a.N) continue;
+                    const int m = mb + q * RPP + lane / LPR;
+                    res[q] = lin_residual<T, 8>(a, m < a.M ? m : a.M - 1, n);
+                }
+            }
+            turn();
+#pragma unroll
+            for (int q = 0; q < 32 / RPP; ++q) {
+                const int rr = q * RPP + lane / LPR, m = mb + rr;
+                if (m < a.M && n < a.N) {
                     float z[8];
                     *reinterpret_cast<f32x4*>(z) = *reinterpret_cast<const f32x4*>(my + rr * LROW + c * 4);
                     *reinterpret_cast<f32x4*>(z + 4) = *reinterpret_cast<const f32x4*>(my + rr * LROW + c * 4 + 16);
@@ -362,22 +398,42 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_kernel(LinArgs a) {
                         *reinterpret_cast<f32x4*>(p) = f32x4{z[0], z[1], z[2], z[3]};
                         *reinterpret_cast<f32x4*>(p + 4) = f32x4{z[4], z[5], z[6], z[7]};
                     } else {
-                        lin_epilogue<T, 8, ACT>(a, m, n, z, bias);
+                        lin_epilogue<T, 8, ACT>(a, m, n, z, bias, res[q]);
                     }
                 }
-            } else {                                               // a lane per column
+            }
+        } else {                                                   // a lane per column
+            const int cc = lane % COLS, n = nb + cc;
+            turn();
+            if (n >= a.N) return;
+#pragma unroll 1
+            for (int q0 = 0; q0 < 32 / RPL; q0 += 8) {             // written out eight rows at a time: all of them overrun the instruction cache
+                LinRow<T, 1> res[8];
+                if (a.residual) {
 #pragma unroll
-                for (int c = 0; c < COLS / 32; c += 2) {
-                    const int cc = 32 * c + lane;
-                    if (cc >= COLS || nb + cc >= a.N) continue;
+                    for (int q = 0; q < 8; ++q) {
+                        const int m = mb + (q0 + q) * RPL + lane / COLS;
+                        res[q] = lin_residual<T, 1>(a, m < a.M ? m : a.M - 1, n);
+                    }
+                }
 #pragma unroll
-                    for (int rr = 0; rr < 32; ++rr)
-                        if (mb + rr < a.M) {
-                            const float z = *reinterpret_cast<const float*>(my + rr * LROW + cc * 4);
-                            lin_epilogue<T, 1, ACT>(a, mb + rr, nb + cc, &z, bias + c / 2);
-                        }
+                for (int q = 0; q < 8; ++q) {
+                    const int rr = (q0 + q) * RPL + lane / COLS, m = mb + rr;
+                    if (m < a.M) {
+                        const float z = *reinterpret_cast<const float*>(my + rr * LROW + cc * 4);
+                        lin_epilogue<T, 1, ACT>(a, m, n, &z, bias, res[q]);
+                    }
                 }
             }
+        }
+    };
+    auto store = [&](auto act) __attribute__((always_inline)) {
+        static_assert(MI == 1 || MI == 2 || MI == 4, "row blocks of a wave");
+        block(std::integral_constant<int, 0>{}, act);
+        if constexpr (MI > 1) block(std::integral_constant<int, 1>{}, act);
+        if constexpr (MI > 2) {
+            block(std::integral_constant<int, 2>{}, act);
+            block(std::integral_constant<int, 3>{}, act);
         }
     };
     if (a.act == kActGelu) store(std::integral_constant<int, kActGelu>{});
@@ -402,8 +458,7 @@ __global__ __launch_bounds__(256) void linear_join_kernel(LinArgs a) {
         for (int e = 0; e < 4; ++e) { z[e] += u[e]; z[4 + e] += v[e]; }
     }
     float bias[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) bias[j] = n + j < a.N ? lin_bias<T>(a, n + j) : 0.f;
+    lin_bias<T, 8>(a, n, bias);
     if (lin_vec(a)) {
         lin_epilogue_any<T, 8>(a, (int)m, n, z, bias);
     } else {
