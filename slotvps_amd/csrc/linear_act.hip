@@ -108,13 +108,14 @@ __device__ __forceinline__ void lin_act(float z, float& y, float& g) {
         y = z > 0.f ? z : z != z ? z : 0.f;
         g = z > 0.f ? 1.f : 0.f;
     } else if constexpr (ACT == kActGelu) {
-        const float zc = fminf(fmaxf(z, -1e18f), 1e18f);           // z * z stays in range, an infinity times zero does not arise
         const float e = __builtin_amdgcn_exp2f(-0.72134752044448170f * z * z);
-        const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f * 0.70710678118654752f, fabsf(zc), 1.f));
+        const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f * 0.70710678118654752f, fabsf(z), 1.f));
+        // q = 0.5 erfc(|z| / sqrt 2); z cdf(z) = max(z, 0) - |z| q
         const float q = e * t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 0.5307027145f, -0.7265760135f), 0.7107068705f), -0.142248368f), 0.127414796f);
-        const float cdf = z > 0.f ? 1.f - q : q;                   // (the half of 0.5 erfc is in the coefficients)
-        y = (z > 0.f ? z : zc) * cdf;
-        g = fmaf(zc * 0.39894228040143268f, e, cdf);
+        const float az = fminf(fabsf(z), 1e18f);                   // q and e are 0 long before: no infinity times zero
+        y = fmaf(-az, q, fmaxf(z, 0.f));                           // (a NaN comes through q)
+        g = z > 0.f ? 1.f - q : q;
+        g = fmaf(copysignf(az, z) * 0.39894228040143268f, e, g);
     }
 }
 
