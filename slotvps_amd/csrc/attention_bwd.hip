@@ -13,40 +13,89 @@
 
 namespace svps {
 
-// L lanes per packed row, 8 channels each (L * 8 >= D)
+// A wave takes 32 packed rows. delta = sum_d dO_id O_id is O's rounding to 16 bits away from sum_j p_ij dP_ij, which the rows of many keys do
+// not notice (dS's own rounding is larger). Rows of few keys do: dS = P * (dP - delta) is then a small difference, of a single visible key
+// zero (2 tokens, 8 / 2 heads of 16, against 64 bits: dQ 3.4 times as far off as its own rounding, as below 1.4 times). Where all keys
+// that a wave's rows see lie within kStatKeys, delta is therefore the second sum, from the same products that dQ and dK repeat.
+constexpr int kStatKeys = 64;
+
 template <typename T, int DP>
 __global__ __launch_bounds__(256) void att_stats_kernel(AttArgs a) {
     typedef typename AttVec<T>::v8 v8;
-    constexpr int L = DP / 8;
-    const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
-    const int lane = (int)(id % L);
-    const long long prow = id / L;
-    const int pairs = a.B * a.Hk;
-    if (prow >= (long long)pairs * a.rows_pad) return;             // whole groups of L lanes
-    const int pair = (int)(prow / a.rows_pad), row = (int)(prow - (long long)pair * a.rows_pad);
+    constexpr int L = DP / 8, PASS = 64 / L, KS = DP / 16;         // L lanes per row with 8 channels each, rows per pass
+    const int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int tiles = a.rows_pad / 128;
+    const int pair = blockIdx.x / tiles, row0 = ((int)blockIdx.x - pair * tiles) * 128 + 32 * w;
     const int b = pair / a.Hk, hk = pair - b * a.Hk;
     const int qlen = att_qlen(a, b), klen = att_klen(a, b);
-    const int n = att_div_g(a, row);
-    const int head = hk * a.G + (row - n * a.G);
-    float s = 0.f;
-    if (n < qlen && 8 * lane < a.D) {
-        const v8 x = *reinterpret_cast<const v8*>((const T*)a.dout + b * a.sdb + n * a.sdn + head * a.sdh + 8 * lane);
-        const v8 y = *reinterpret_cast<const v8*>((const T*)a.out_in + (((long long)b * a.N + n) * a.H + head) * a.D + 8 * lane);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) s += (float)x[j] * (float)y[j];
-    }
-#pragma unroll
-    for (int o = 1; o < L; o <<= 1) s += __shfl_xor(s, o);
-    if (lane == 0) {
-        int lo = 0, hi = 0;
-        float lse2 = INFINITY;                                     // exp2(. - inf) = 0: rows behind qlen and rows that see nothing
-        if (n < qlen) {
+    const int n0 = att_div_g(a, row0);
+    float delta = 0.f, lse2 = INFINITY;                            // of row row0 + r; exp2(. - inf) = 0: rows behind qlen and rows that see nothing
+    int lo = 0, hi = 0;
+    if (n0 < qlen) {
+        const int row = row0 + r, n = att_div_g(a, row), head = hk * a.G + (row - n * a.G);
+        const bool have = n < qlen;
+        if (have) {
             att_range(a, n, qlen, klen, lo, hi);
             const float x = a.lse[((long long)b * a.H + head) * a.N + n];
             if (x != -INFINITY) lse2 = x * kLog2e;
         }
+        int n1 = att_div_g(a, row0 + 31), lo_min, hi_max, tmp;
+        n1 = n1 < qlen ? n1 : qlen - 1;
+        att_range(a, n0, qlen, klen, lo_min, tmp);
+        att_range(a, n1, qlen, klen, tmp, hi_max);
+        if (hi_max - lo_min <= kStatKeys) {
+            const T* qp = (const T*)a.q + b * a.sqb + n * a.sqn + head * a.sqh;
+            const T* dp = (const T*)a.dout + b * a.sdb + n * a.sdn + head * a.sdh;
+            const T* kp = (const T*)a.k + b * a.skb + hk * a.skh;
+            const T* vp = (const T*)a.v + b * a.svb + hk * a.svh;
+            const float c = a.scale * kLog2e;
+            auto piece = [&](const T* x, bool on, int d) __attribute__((always_inline)) {
+                u32x4 y = {0, 0, 0, 0};
+                if (on && d < a.D) y = *reinterpret_cast<const u32x4*>(x + d);
+                return __builtin_bit_cast(v8, y);
+            };
+            for (int k0 = lo_min; k0 < hi_max; k0 += 32) {
+                const int kr = k0 + r < hi_max ? k0 + r : hi_max - 1;
+                f32x16 s, g;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) { s[i] = 0.f; g[i] = 0.f; }
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    const int d = 16 * ks + 8 * h;
+                    s = mfma16(piece(kp + kr * a.skn, true, d), piece(qp, have, d), s);
+                    g = mfma16(piece(vp + kr * a.svn, true, d), piece(dp, have, d), g);
+                }
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int key = k0 + acc_row(i, h);
+                    const float t = __builtin_amdgcn_exp2f(fmaf(s[i], c, -lse2)) * g[i];
+                    delta += key >= lo && key < hi ? t : 0.f;
+                }
+            }
+            delta += __shfl_xor(delta, 32);
+        } else {
+#pragma unroll 4
+            for (int q = 0; q < 32; q += PASS) {
+                const int rr = row0 + q + lane / L, m = att_div_g(a, rr), hd = hk * a.G + (rr - m * a.G), d = 8 * (lane % L);
+                float t = 0.f;
+                if (m < qlen && d < a.D) {
+                    const v8 x = *reinterpret_cast<const v8*>((const T*)a.dout + b * a.sdb + m * a.sdn + hd * a.sdh + d);
+                    const v8 y = *reinterpret_cast<const v8*>((const T*)a.out_in + (((long long)b * a.N + m) * a.H + hd) * a.D + d);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) t += (float)x[j] * (float)y[j];
+                }
+#pragma unroll
+                for (int o = 1; o < L; o <<= 1) t += __shfl_xor(t, o);
+                t = __shfl(t, ((r - q) & (PASS - 1)) * L);          // row q + i stands in lanes L i ..
+                if (r >= q && r < q + PASS) delta = t;
+            }
+        }
+    }
+    if (h == 0) {
+        const long long prow = (long long)pair * a.rows_pad + row0 + r;
         a.stat_lse2[prow] = lse2;
-        a.stat_delta[prow] = s;
+        a.stat_delta[prow] = delta;
         a.stat_lo[prow] = lo;
         a.stat_hi[prow] = hi;
     }
@@ -455,8 +504,8 @@ static int attention_bwd_launch(const AttArgs& a, const AttBwdPlan& p, hipStream
     constexpr int LDS = 2 * (2 * 64 * DP * 2 + 512) + (DP == 128 ? 8192 : 0);     // two pairs of 64-row tiles; for dK and dV their (lse, delta) and kept fragments
     hipError_t e = attr.ensure((const void*)att_bwd_kernel<T, DP>, LDS);
     if (e != hipSuccess) return (int)e;
-    const long long pairs = (long long)a.B * a.Hk, lanes = pairs * a.rows_pad * (DP / 8);
-    hipLaunchKernelGGL((att_stats_kernel<T, DP>), dim3((unsigned)((lanes + 255) / 256)), dim3(256), 0, stream, a);
+    const long long pairs = (long long)a.B * a.Hk;
+    hipLaunchKernelGGL((att_stats_kernel<T, DP>), dim3((unsigned)(pairs * (a.rows_pad / 128))), dim3(256), 0, stream, a);
     e = hipGetLastError();
     if (e != hipSuccess) return (int)e;
     const unsigned grid = (unsigned)(pairs * ((long long)a.k_tiles * a.k_splits + (long long)a.tiles * a.splits));

@@ -244,6 +244,28 @@ def test_attention_long_and_split(cuda):
         _close(a, r, 4 * t, name)
 
 
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("N,M,H,Hk,D,frame,window", [(5, 5, 4, 2, 64, 1, 0), (70, 1, 2, 2, 32, 0, 0), (200, 200, 4, 1, 128, 1, 1), (33, 90, 3, 3, 40, 1, 1)])
+def test_attention_gradient_of_one_visible_key(cuda, N, M, H, Hk, D, frame, window, dt):
+    """A row that sees a single key has p = 1 whatever q and k are: its dS, and so its dQ, is zero but for fp32 rounding.
+    |dS| <= p |dP - delta|: dP and delta are D fp32 additions of the same products, 2 D 2^-24 S with S = sum_d |dO_d v_d|, and p is off by
+    2^-19 at |s| < 8 (three roundings of a number below 16 in front of exp2): together below (2 D + 32) 2^-24 S, times 1 + 2^-6 for the
+    roundings of dS and dQ to 16 bits. fp16 cannot hold less than 2^-25 of either."""
+    B = 2
+    q, k, v, do = _rand((B, N, H, D), dt, 41, cuda), _rand((B, M, Hk, D), dt, 42, cuda), _rand((B, M, Hk, D), dt, 43, cuda), _rand((B, N, H, D), dt, 44, cuda)
+    out, lse = ops.attention(q, k, v, frame=frame, window=window, return_lse=True)
+    dq = ops.attention_bwd(do, q, k, v, out, lse, frame=frame, window=window)[0]
+    for n in range(N):
+        one = n + M - N if frame else 0                                    # the only key that row n sees, if it does see only one
+        if (window != 1 and M > 1 and one != 0) or one < 0:
+            continue
+        kk, vv = k[:, one].repeat_interleave(H // Hk, 1).double(), v[:, one].repeat_interleave(H // Hk, 1).double()
+        assert (q[:, n].double() * kk).sum(-1).abs().max() * D ** -0.5 < 8
+        S = (do[:, n].double() * vv).abs().sum(-1, keepdim=True)
+        tol = (2 * D + 32) * 2.0 ** -24 * S * D ** -0.5 * kk.abs() * (1 + 2.0 ** -6) + 2.0 ** -25 * (1 + kk.abs())
+        assert (dq[:, n].double().abs() <= tol).all(), f"token {n}: {float((dq[:, n].double().abs() - tol).max()):.3e} over"
+
+
 def test_attention_views_strides_and_broadcast(cuda):
     B, N, H, Hk, D = 2, 70, 4, 2, 64
     qkv = _rand((B, N, H + 2 * Hk, D), BF, 1, cuda)
