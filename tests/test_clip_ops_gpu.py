@@ -583,3 +583,34 @@ def test_refusals(cuda):
     ]:
         with pytest.raises(err):
             fn()
+
+
+def test_views_whose_offsets_pass_32_bits(cuda):
+    """Tokens that lie 40 MB apart (a slice of a memory of many layers) and rows of almost 2^22 channels: the bits are those of packed copies."""
+    n = 130
+    far = torch.empty(n, 20 << 20, dtype=BF, device=cuda)
+    def view(i, heads, d):
+        x = far[:, 8192 * i:8192 * i + heads * d]
+        x.copy_(_rand((n, heads * d), BF, 51 + i, cuda))
+        return x.unflatten(1, (heads, d))[None]
+    q, k, v, do = view(0, 4, 64), view(1, 2, 64), view(2, 2, 64), view(3, 4, 64)
+    assert k.stride(1) * (n - 1) * 2 > 1 << 32
+    near = [t.contiguous() for t in (q, k, v, do)]
+    for kw in (dict(), dict(frame=1)):
+        out, lse = ops.attention(q, k, v, return_lse=True, **kw)
+        ref, rlse = ops.attention(*near[:3], return_lse=True, **kw)
+        assert torch.equal(out, ref) and torch.equal(lse, rlse)
+        got, want = ops.attention_bwd(do, q, k, v, out, lse, **kw), ops.attention_bwd(near[3], *near[:3], ref, rlse, **kw)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    pos = torch.arange(n, device=cuda)[:, None]
+    assert all(torch.equal(a, b) for a, b in zip(ops.rotary_axes(q, pos, (64,), also=k), ops.rotary_axes(near[0], pos, (64,), also=near[1])))
+    del far, q, k, v, do
+    wide = torch.empty(600, (1 << 22) - 8, dtype=BF, device=cuda)
+    x, w = wide[:, :136], wide[:200, 4096:4096 + 136]
+    x.copy_(_rand((600, 136), BF, 61, cuda))
+    w.copy_(_rand((200, 136), BF, 62, cuda))
+    dy = wide[:, 8192:8192 + 200]
+    dy.copy_(_rand((600, 200), BF, 63, cuda))
+    assert torch.equal(ops.linear_act(x, w), ops.linear_act(x.contiguous(), w.contiguous()))
+    got, want = ops.linear_act_bwd(dy, x, w)[:2], ops.linear_act_bwd(dy.contiguous(), x.contiguous(), w.contiguous())[:2]
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
