@@ -8,6 +8,13 @@
 // That is 7 matrix products for the 5 of one joint kernel; the joint form would add dQ from many workgroups with atomics, whose order
 // changes the result, or write every dS to memory (2 bytes per visible pair and head).
 // Few tiles on either side: the walked range is split over workgroups that leave fp32 partial sums, added by att_add_kernel.
+//
+// P and dS are rounded to 16 bits once each, as operands of the products with dO, Q and K: beside the roundings of q, k, v and of the result
+// they make a gradient 1.4 times as far off as its own rounding. Everything else is fp32.
+//
+// Bound: the matrix products (10 D flop per visible pair, 14 D executed). Measured in bf16, all launches, flop counted as 10 D: 4 x 4096
+// tokens, 16 heads of 128 1.84 ms = 747 TFLOP/s, causal over 4 key heads 0.97 ms = 707; 10240 tokens, 8 heads of 64 0.88 ms = 610, of 32
+// 0.54 ms = 497 TFLOP/s; 5 x 100 tokens, 8 heads of 32 10.4 us.
 #include "attention.h"
 #include "../../include/slotvps_hip.h"
 

@@ -8,11 +8,16 @@
 // one rounding of y. The slope g is stored instead of the pre-activation: held as int16 in units of 2^-14 it is off by 3e-5 (a 16-bit
 // pre-activation in bf16: by up to 4e-3 times the curvature), and the backward pass needs no transcendental.
 //
-// Tile BM x BN x 64, WM x WN waves; LDS double-buffered by 16-byte LDS-DMA, one barrier per 64-deep step. The W fragment is the MFMA's row
-// operand: a lane owns one row m and four consecutive n per accumulator quad. Tiles behind each other in memory go to one XCD (its L2
+// Tile BM x BN x 64, WM x WN waves; operand tiles come by 16-byte LDS-DMA, the next ones while this one is multiplied. The W fragment is the
+// MFMA's row operand: a lane owns one row m and four consecutive n per accumulator quad. Tiles behind each other in memory go to one XCD (its L2
 // holds the shared operand rows). Few tiles: the k range is split over workgroups, fp32 partial sums are added in order (same epilogue).
 //
 // Operands whose rows do not start on 16 bytes or whose length is no multiple of 8 are first copied with zero-padded rows (linear_pack).
+//
+// Bound: matrix instructions, from about 1000 columns on; they run at the clock that the power allows (8192 cubed with operands of zeros:
+// 600 us). Measured in bf16: 8192 cubed 805 us = 1365 TFLOP/s, dx 820 us, dW 855 us; 10240 x 6144 -> 1536 165 us = 1170 TFLOP/s. Narrower ones
+// by their bytes and the epilogue: 32768 x 384 -> 1536 58 us, with GELU 78 us (12 vector and 2 transcendental instructions per value, which
+// with one workgroup per CU nothing runs under). A few rows by the latency of one pass over the weights.
 #include <type_traits>
 
 #include "attention.h"
@@ -99,7 +104,7 @@ __device__ __forceinline__ typename AttVec<T>::v8 lin_frag(const char* lds, int 
 // GELU through the complementary error function's exponential form (Abramowitz and Stegun 7.1.26, |error| <= 1.5e-7):
 //   erfc(x) = exp(-x^2) t (a1 + t (a2 + t (a3 + t (a4 + t a5)))), t = 1 / (1 + p x), x = |z| / sqrt 2
 // with exp(-x^2) = exp(-z^2 / 2), the same exponential that the slope needs: one exponential and one reciprocal per value in place of
-// erff's two branches (measured at 32768 x 384 -> 1536: 154 us with erff, 96 us so).
+// erff's two branches (32768 x 384 -> 1536, when the whole took 96 us: 154 us with erff).
 template <int ACT>
 __device__ __forceinline__ void lin_act(float z, float& y, float& g) {
     y = z;
@@ -145,7 +150,7 @@ __device__ __forceinline__ void lin_bias(const LinArgs& a, int n, float* b) {
 
 // N8 consecutive columns n .. of row m (8: N % 8 == 0 and 16-byte aligned tensors; 1: any): their residual, asked for on its own so that a
 // caller with several rows has all of them on the way before its first store (a load after a store waits for both; 40001 x 256 -> 333:
-// 61 us row by row)
+// 61 us row by row, 36 us so)
 template <typename T, int N8> struct LinRow;
 template <typename T> struct LinRow<T, 8> { typename AttVec<T>::v8 r; };
 template <typename T> struct LinRow<T, 1> { T r[1]; };

@@ -1401,7 +1401,9 @@ def attention(q, k, v, q_lens=None, k_lens=None, frame=0, window=0, scale=None, 
 
 def attention_bwd(dout, q, k, v, out, lse, q_lens=None, k_lens=None, frame=0, window=0, scale=None):
     """Gradients (dq, dk, dv) of attention as a plain call, from the forward's out and lse and the same other arguments. The probabilities
-    are computed again; sums run in a fixed order (two calls give the same bits). Rows and keys behind the lengths get zeros."""
+    are computed again; sums run in a fixed order (two calls give the same bits). Rows and keys behind the lengths get zeros.
+    In fp16 dS = P (dout v^T - delta) passes through fp16 as an operand: beyond 65504 it overflows, below 6e-8 it vanishes - scale the loss
+    as fp16 training does anyway."""
     q, k, v, cfg = _att_args(q, k, v, q_lens, k_lens, frame, window, scale)
     return _att_bwd(dout, q, k, v, out, lse, *cfg)
 
