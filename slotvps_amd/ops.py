@@ -1159,8 +1159,31 @@ def _no_capture(what):
 
 @functools.lru_cache(maxsize=512)
 def _plan_bytes(fn, device, *sizes):
-    """Workspace of a launch by its sizes alone (the plan asks for the device's CU count: called with that device current)."""
-    return getattr(_lib.load(), fn)(*sizes)
+    """Workspace of a launch by its sizes alone (the plan asks for the current device's CU count)."""
+    with torch.cuda.device(device):
+        return getattr(_lib.load(), fn)(*sizes)
+
+
+def _one_device(first, *others):
+    """The device index of a call's tensors (None: absent); they must share it."""
+    dev = first.device
+    for t in others:
+        if t is not None and t.device != dev:
+            raise ValueError(f"tensor arguments on different devices: {sorted({str(x.device) for x in (first, *others) if x is not None})}")
+    return dev.index
+
+
+def _launch(name, device, *args):
+    """One C-ABI call with its device current, on that device's current stream: what _on does, without an object (small calls are the
+    interpreter's time)."""
+    fn = getattr(_lib.load(), name)
+    if device == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(device))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(device))
+    if rc:
+        _lib.check(rc, name)
 
 
 @functools.lru_cache(maxsize=64)
@@ -1176,10 +1199,16 @@ def _rotary_table(split, base, ladder):
     return (ctypes.c_int * len(split))(*split), (ctypes.c_double * len(turns))(*turns)
 
 
-def _rotary_args(x, positions, split, base, pairing, ladder, also):
+@functools.lru_cache(maxsize=256)
+def _rotary_split(*split):
     split = tuple(int(d) for d in split)
     if not 1 <= len(split) <= 4 or any(d < 2 or d % 2 for d in split):
         raise ValueError(f"rotary_axes: split must be one to four even channel counts, got {split}")
+    return split, sum(split)
+
+
+def _rotary_args(x, positions, split, base, pairing, ladder, also):
+    split, turning = _rotary_split(*split)
     if pairing not in ("half", "adjacent") or ladder not in ("axis", "shared"):
         raise ValueError("rotary_axes: pairing is 'half' or 'adjacent', ladder is 'axis' or 'shared'")
     if not (base > 0.0 and math.isfinite(base)):
@@ -1188,7 +1217,7 @@ def _rotary_args(x, positions, split, base, pairing, ladder, also):
     if x.dim() != 4:
         raise ValueError(f"rotary_axes: x is [B, N, H, D], got {tuple(x.shape)}")
     B, N, _, D = x.shape
-    if sum(split) > min(D, 256):
+    if turning > min(D, 256):
         raise ValueError(f"rotary_axes: split {split} needs more than the {min(D, 256)} channels that can turn")
     if D > 4096:
         raise ValueError("rotary_axes: at most 4096 channels per head")
@@ -1216,17 +1245,16 @@ def _rotary_launch(x, positions, split, base, pairing, ladder, also, inverse):
         return y, y2
     if B == 0 or N == 0 or H == 0:
         return y, y2
-    lib = _lib.load()
     csplit, turns = _rotary_table(split, float(base), ladder)
     ps = positions.stride()
-    psb, psn = (0, ps[0]) if positions.dim() == 2 else (ps[0], ps[1])
-    with _on(x, positions, also, y, y2) as ctx:
-        rc = lib.svps_rotary_axes(x.data_ptr(), _ll3(*x.stride()[:3]), y.data_ptr(), H,
-                                  _at(also), None if also is None else _ll3(*also.stride()[:3]), None if also is None else y2.data_ptr(),
-                                  0 if also is None else also.shape[2],
-                                  positions.data_ptr(), psb, psn, _POS_CODE[positions.dtype], len(split), csplit, turns,
-                                  0 if pairing == "half" else 1, int(inverse), _DTYPE_CODE[x.dtype], B, N, D, ctx.stream)
-    _lib.check(rc, "svps_rotary_axes")
+    psb, psn = (0, ps[0]) if len(ps) == 2 else (ps[0], ps[1])
+    if also is None:
+        second = (None, None, None, 0)
+    else:
+        second = (also.data_ptr(), _ll3(*also.stride()[:3]), y2.data_ptr(), also.shape[2])
+    _launch("svps_rotary_axes", _one_device(x, positions, also), x.data_ptr(), _ll3(*x.stride()[:3]), y.data_ptr(), H, *second,
+            positions.data_ptr(), psb, psn, _POS_CODE[positions.dtype], len(split), csplit, turns,
+            0 if pairing == "half" else 1, int(inverse), _DTYPE_CODE[x.dtype], B, N, D)
     return y, y2
 
 
@@ -1327,14 +1355,11 @@ def _att_fwd(q, k, v, q_lens, k_lens, frame, window, scale, want_lse):
         if lse is not None:
             lse.fill_(float("-inf"))
         return out, lse
-    lib = _lib.load()
-    with _on(q, k, v, out, lse, q_lens, k_lens) as ctx:
-        nbytes = _plan_bytes("svps_attention_workspace_bytes", ctx.device.index, B, N, M, H, Hk, D)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-        rc = lib.svps_attention_fwd(q.data_ptr(), _att_strides(q), k.data_ptr(), _att_strides(k), v.data_ptr(), _att_strides(v),
-                                    out.data_ptr(), _at(lse), _at(q_lens), _at(k_lens), _at(ws), nbytes, B, N, M, H, Hk, D,
-                                    frame, window, scale, _DTYPE_CODE[q.dtype], ctx.stream)
-    _lib.check(rc, "svps_attention_fwd")
+    dev = _one_device(q, k, v, q_lens, k_lens)
+    nbytes = _plan_bytes("svps_attention_workspace_bytes", dev, B, N, M, H, Hk, D)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    _launch("svps_attention_fwd", dev, q.data_ptr(), _att_strides(q), k.data_ptr(), _att_strides(k), v.data_ptr(), _att_strides(v),
+            out.data_ptr(), _at(lse), _at(q_lens), _at(k_lens), _at(ws), nbytes, B, N, M, H, Hk, D, frame, window, scale, _DTYPE_CODE[q.dtype])
     return out, lse
 
 
@@ -1351,15 +1376,12 @@ def _att_bwd(dout, q, k, v, out, lse, q_lens, k_lens, frame, window, scale):
     dq, dk, dv = new((B, N, H, D)), new((B, M, Hk, D)), new((B, M, Hk, D))
     if empty:
         return dq, dk, dv
-    lib = _lib.load()
-    with _on(dout, q, k, v, out, lse, q_lens, k_lens) as ctx:
-        nbytes = _plan_bytes("svps_attention_bwd_workspace_bytes", ctx.device.index, B, N, M, H, Hk, D)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-        rc = lib.svps_attention_bwd(dout.data_ptr(), _att_strides(dout), q.data_ptr(), _att_strides(q), k.data_ptr(), _att_strides(k),
-                                    v.data_ptr(), _att_strides(v), out.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-                                    _at(q_lens), _at(k_lens), ws.data_ptr(), nbytes, B, N, M, H, Hk, D, frame, window, scale,
-                                    _DTYPE_CODE[q.dtype], ctx.stream)
-    _lib.check(rc, "svps_attention_bwd")
+    dev = _one_device(dout, q, k, v, out, lse, q_lens, k_lens)
+    nbytes = _plan_bytes("svps_attention_bwd_workspace_bytes", dev, B, N, M, H, Hk, D)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    _launch("svps_attention_bwd", dev, dout.data_ptr(), _att_strides(dout), q.data_ptr(), _att_strides(q), k.data_ptr(), _att_strides(k),
+            v.data_ptr(), _att_strides(v), out.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _at(q_lens), _at(k_lens),
+            ws.data_ptr(), nbytes, B, N, M, H, Hk, D, frame, window, scale, _DTYPE_CODE[q.dtype])
     return dq, dk, dv
 
 
@@ -1458,14 +1480,12 @@ def _linear_fwd(x, weight, bias, act, residual, want_gate):
         return y, gate
     x2 = _rows16(x, "x", x.dtype, K)
     M = x2.shape[0]
-    lib = _lib.load()
-    with _on(x, weight, bias, residual) as ctx:
-        ldx, ldw, px, pw = _ld(x2), _ld(weight), x2.data_ptr(), weight.data_ptr()
-        nbytes = _plan_bytes("svps_linear_act_workspace_bytes", ctx.device.index, M, K, N, ldx, ldw, (px | pw) & 15)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
-        rc = lib.svps_linear_act_fwd(px, ldx, pw, ldw, _at(bias), int(bias is not None and bias.dtype == torch.float32), _at(residual), act,
-                                     y.data_ptr(), _at(gate), _at(ws), nbytes, M, K, N, _DTYPE_CODE[x.dtype], ctx.stream)
-    _lib.check(rc, "svps_linear_act_fwd")
+    dev = _one_device(x, weight, bias, residual)
+    ldx, ldw, px, pw = _ld(x2), _ld(weight), x2.data_ptr(), weight.data_ptr()
+    nbytes = _plan_bytes("svps_linear_act_workspace_bytes", dev, M, K, N, ldx, ldw, (px | pw) & 15)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+    _launch("svps_linear_act_fwd", dev, px, ldx, pw, ldw, _at(bias), int(bias is not None and bias.dtype == torch.float32), _at(residual), act,
+            y.data_ptr(), _at(gate), _at(ws), nbytes, M, K, N, _DTYPE_CODE[x.dtype])
     return y, gate
 
 
@@ -1482,16 +1502,13 @@ def _linear_bwd(dy, x, weight, gate, bias, want_dx, want_dw):
         return dx, dw, db
     x2, dy2 = _rows16(x, "x", x.dtype, K), _rows16(dy, "dy", x.dtype, N)
     M = dy2.shape[0]
-    lib = _lib.load()
-    with _on(dy, x, weight, gate, bias) as ctx:
-        ldy, ldx, ldw = _ld(dy2), _ld(x2), _ld(weight)
-        nbytes = _plan_bytes("svps_linear_act_bwd_workspace_bytes", ctx.device.index, M, K, N, ldy, ldx, ldw,
-                             (x2.data_ptr() | weight.data_ptr() | dy2.data_ptr()) & 15, int(gate is not None), int(want_dx), int(want_dw),
-                             int(db is not None))
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
-        rc = lib.svps_linear_act_bwd(dy2.data_ptr(), ldy, x2.data_ptr(), ldx, weight.data_ptr(), ldw, _at(gate), _at(dx), _at(dw), _at(db),
-                                     int(db is not None and db.dtype == torch.float32), _at(ws), nbytes, M, K, N, _DTYPE_CODE[x.dtype], ctx.stream)
-    _lib.check(rc, "svps_linear_act_bwd")
+    dev = _one_device(dy, x, weight, gate, bias)
+    ldy, ldx, ldw, pd, px, pw = _ld(dy2), _ld(x2), _ld(weight), dy2.data_ptr(), x2.data_ptr(), weight.data_ptr()
+    nbytes = _plan_bytes("svps_linear_act_bwd_workspace_bytes", dev, M, K, N, ldy, ldx, ldw, (px | pw | pd) & 15, int(gate is not None),
+                         int(want_dx), int(want_dw), int(db is not None))
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+    _launch("svps_linear_act_bwd", dev, pd, ldy, px, ldx, pw, ldw, _at(gate), _at(dx), _at(dw), _at(db),
+            int(db is not None and db.dtype == torch.float32), _at(ws), nbytes, M, K, N, _DTYPE_CODE[x.dtype])
     return dx, dw, db
 
 
