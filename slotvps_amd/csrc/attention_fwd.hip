@@ -283,11 +283,15 @@ struct AttPlan { int nw, rb, kt, tiles, splits; };
 
 // One wave of 32 rows where that is all there are. Above, four waves: of one row block each, or of two at heads above 64,
 // where a fragment read then serves two products and the registers allow it (4 x 4096 tokens, 16 heads of 128: 642 us with one, 560 us with
-// two; heads of 64: 293 and 398 us), if the workgroups are enough for four rounds. The keys are split where CUs would stand idle.
+// two; heads of 64: 293 and 398 us), if the workgroups are enough for four rounds. Eight waves at heads of
+// 33 to 64, halving the requests for keys, where that leaves the CUs as evenly filled (4 x 4096 tokens, 16 heads of 64: 334 us with four, 312
+// with eight; 10240 tokens, 8 heads, 640 or 320 workgroups on 256 CUs: 285 and 320 us; with two waves 570 and 395). The keys are split
+// where CUs would stand idle.
 static AttPlan attention_plan(int B, int N, int M, int H, int Hk, int D) {
     const long long rows = (long long)N * (H / Hk), pairs = (long long)B * Hk, cus = svps_num_cus();
     AttPlan p;
-    p.nw = rows <= 32 ? 1 : 4;
+    auto filled = [&](int nw) { return nw * ((pairs * ((rows + 32 * nw - 1) / (32 * nw)) + cus - 1) / cus); };     // waves on the fullest CU
+    p.nw = rows <= 32 ? 1 : D > 32 && D <= 64 && filled(8) <= filled(4) ? 8 : 4;
     p.rb = D > 64 && pairs * ((rows + 255) / 256) >= 4 * cus ? 2 : 1;
     p.kt = p.nw == 1 ? 32 : 64;
     p.tiles = (int)((rows + 32 * p.nw * p.rb - 1) / (32 * p.nw * p.rb));
@@ -316,6 +320,8 @@ static int attention_variant(const AttArgs& a, const AttPlan& p, hipStream_t str
     if (p.nw == 1) return attention_launch<T, DP, 1, 32, 1>(a, stream);
     if constexpr (DP == 128)
         if (p.rb == 2) return attention_launch<T, DP, 4, 64, 2>(a, stream);
+    if constexpr (DP == 64)
+        if (p.nw == 8) return attention_launch<T, DP, 8, 64, 1>(a, stream);
     return attention_launch<T, DP, 4, 64, 1>(a, stream);
 }
 

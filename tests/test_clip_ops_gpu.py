@@ -244,6 +244,25 @@ def test_attention_long_and_split(cuda):
         _close(a, r, 4 * t, name)
 
 
+@pytest.mark.parametrize("frame,window", [(0, 0), (1, 0), (50, 2)])
+@pytest.mark.parametrize("D", [64, 40])
+def test_attention_of_many_full_workgroups(cuda, D, frame, window):
+    """Batches whose rows fill workgroups of 256 rows on every compute unit, with rows and keys behind the lengths."""
+    B, N, M, H, Hk = 32, 250, 203, 16, 8
+    ql, kl = [N - 3 * b for b in range(B)], [M - 5 * b for b in range(B)]
+    q, k, v, do = _rand((B, N, H, D), BF, 1, cuda), _rand((B, M, Hk, D), BF, 2, cuda), _rand((B, M, Hk, D), BF, 3, cuda), _rand((B, N, H, D), BF, 4, cuda)
+    for b in range(B):
+        q[b, ql[b]:], do[b, ql[b]:], k[b, kl[b]:], v[b, kl[b]:] = math.nan, math.inf, math.nan, -math.inf
+    kw = dict(q_lens=_lens(ql, B, N, cuda), k_lens=_lens(kl, B, M, cuda), frame=frame, window=window)
+    out, lse = ops.attention(q, k, v, return_lse=True, **kw)
+    ref, tol = _attention_ref(q, k, v, do, ql, kl, frame, window, D ** -0.5, BF)
+    _close(out, ref[0], tol[0], "out")
+    none = torch.isinf(ref[1])
+    assert torch.equal(torch.isinf(lse), none) and (lse.double() - ref[1])[~none].abs().max() < 1e-3
+    for name, a, r, t in zip(("dq", "dk", "dv"), ops.attention_bwd(do, q, k, v, out, lse, **kw), ref[2:], tol[1:]):
+        _close(a, r, t, name)
+
+
 @pytest.mark.parametrize("dt", [BF, HF])
 @pytest.mark.parametrize("N,M,H,Hk,D,frame,window", [(5, 5, 4, 2, 64, 1, 0), (70, 1, 2, 2, 32, 0, 0), (200, 200, 4, 1, 128, 1, 1), (33, 90, 3, 3, 40, 1, 1)])
 def test_attention_gradient_of_one_visible_key(cuda, N, M, H, Hk, D, frame, window, dt):
