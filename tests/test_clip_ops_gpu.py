@@ -633,3 +633,20 @@ def test_views_whose_offsets_pass_32_bits(cuda):
     assert torch.equal(ops.linear_act(x, w), ops.linear_act(x.contiguous(), w.contiguous()))
     got, want = ops.linear_act_bwd(dy, x, w)[:2], ops.linear_act_bwd(dy.contiguous(), x.contiguous(), w.contiguous())[:2]
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("c", [8, 64, 72, 136, 192, 264])
+def test_linear_act_short_sums_over_wide_results(cuda, c):
+    """One to five steps of the contraction over results of 4100 x 4088, in each of the three products. Tolerance: c fp32 additions (c 2^-24 of
+    the absolute sum, twice that for the products' own order) and half a step of bf16."""
+    big, wide = 4100, 4088
+    def check(got, a, b):                                            # got = a b^T over c columns
+        a, b = a.double(), b.double()
+        ref, mass = a @ b.t(), a.abs() @ b.abs().t()
+        _close(got, ref, 2 * c * 2.0 ** -24 * mass + 2.0 ** -8 * ref.abs(), f"{tuple(got.shape)} over {c}")
+    x, w = _rand((big, c), BF, 71, cuda), _rand((wide, c), BF, 72, cuda)
+    check(ops.linear_act(x, w), x, w)
+    dy, w = _rand((big, c), BF, 73, cuda), _rand((c, wide), BF, 74, cuda)
+    check(ops.linear_act_bwd(dy, _rand((big, wide), BF, 75, cuda), w, want_dw=False)[0], dy, w.t())
+    dy, x = _rand((c, big), BF, 76, cuda), _rand((c, wide), BF, 77, cuda)
+    check(ops.linear_act_bwd(dy, x, _rand((big, wide), BF, 78, cuda), want_dx=False)[1], dy.t(), x.t())
