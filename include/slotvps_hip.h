@@ -555,6 +555,7 @@ int svps_mask_decode_f32_fwd(const float* feat, const float* embed, const float*
  *   qlens / klens [B] int32 device arrays or NULL (all rows valid), clamped to [0, N] / [0, M]; nothing behind a length is read.
  *   Visible: frame = 0 every key of the entry; frame > 0: with p = n + klen - qlen, keys j with j / frame <= floor(p / frame), window > 0:
  *   and more than floor(p / frame) - window. Rows behind qlen and rows that see nothing: out 0, lse -inf.
+ *   Rows that see a NaN or +inf score, or only -inf: out NaN.
  *   D % 8 == 0, D <= 128; scale > 0; tensors aligned to 16 bytes, strides multiples of 8 elements. bf16 / fp16.
  * svps_attention_bwd: dq, dk, dv (contiguous) from dout and the forward's out (contiguous) and lse, all rows written (zeros where nothing
  *   flows). Sums in a fixed order: two calls give the same bits.

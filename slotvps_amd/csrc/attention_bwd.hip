@@ -44,8 +44,7 @@ __global__ __launch_bounds__(256) void att_stats_kernel(AttArgs a) {
         const bool have = n < qlen;
         if (have) {
             att_range(a, n, qlen, klen, lo, hi);
-            const float x = a.lse[((long long)b * a.H + head) * a.N + n];
-            if (x != -INFINITY) lse2 = x * kLog2e;
+            if (lo < hi) lse2 = a.lse[((long long)b * a.H + head) * a.N + n] * kLog2e;
         }
         int n1 = att_div_g(a, row0 + 31), lo_min, hi_max, tmp;
         n1 = n1 < qlen ? n1 : qlen - 1;
@@ -86,7 +85,7 @@ __global__ __launch_bounds__(256) void att_stats_kernel(AttArgs a) {
             }
             delta += __shfl_xor(delta, 32);
             sum += __shfl_xor(sum, 32);
-            delta = sum > 0.f ? delta / sum : 0.f;                 // the sum is 1 but for the roundings of lse: of one key, delta is dP to the bit
+            delta = sum == 0.f ? 0.f : delta / sum;                // the sum is 1 but for the roundings of lse: of one key, delta is dP to the bit
         } else {
 #pragma unroll 4
             for (int q = 0; q < 32; q += PASS) {

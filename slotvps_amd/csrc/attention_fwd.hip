@@ -199,7 +199,10 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
         if (n >= m.N) continue;
         const long long orow = ((long long)b * m.N + n) * m.H + head;
         const float sum = wave_half_xor_sum(l[i]);
-        const bool some = n < qlen && sum > 0.f;
+        // by the interval, not by the sum: that is NaN where a visible score is, and such a row must not pass for one that sees nothing
+        int lo, hi;
+        att_range(m, n < qlen ? n : qlen - 1, qlen, klen, lo, hi);
+        const bool some = n < qlen && lo < hi;
         if (m.splits > 1) {
             const long long rows = (long long)m.B * m.N * m.H;
             float* po = m.part + (split * rows + orow) * m.D;
@@ -208,7 +211,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
             if (h == 0) {
                 float* ml = m.part + (long long)m.splits * rows * m.D + (split * rows + orow) * 2;
                 ml[0] = mc[i];
-                ml[1] = some ? sum : 0.f;
+                ml[1] = some ? sum : -1.f;
             }
             continue;
         }
@@ -226,6 +229,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP == 1
 
 // joins the splits of a row: o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s. One workgroup per row: every lane of a wave holds the
 // weight of one split (splits <= 64), thread (g, c) adds splits g, g + 8, .. of channels 4 c .. 4 c + 3, the eight sums meet in LDS.
+// l_s is 0 where the row sees none of a split's keys, negative in every split where it sees no key at all, and NaN where a score is.
 template <typename T>
 __global__ __launch_bounds__(256) void attention_combine_kernel(AttArgs a) {
     __shared__ float red[8][128];
@@ -238,13 +242,14 @@ __global__ __launch_bounds__(256) void attention_combine_kernel(AttArgs a) {
     if (lane < a.splits) {
         const float2 x = *reinterpret_cast<const float2*>(ml + (lane * rows + row) * 2);
         ls = x.y;
-        ms = ls > 0.f ? x.x : -INFINITY;
+        if (!(ls <= 0.f)) ms = x.x;
     }
+    const bool none = __shfl(ls, 0) < 0.f;
     float m = ms;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
-    const float f = ls > 0.f ? exp2f(ms - m) : 0.f;
-    float l = f * ls;
+    const float f = ls <= 0.f ? -1.f : exp2f(ms - m);              // -1: the split has no part in the row
+    float l = ls <= 0.f ? 0.f : f * ls;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) l += __shfl_xor(l, o);
     if (threadIdx.x < 64) wt[lane] = f;
@@ -254,7 +259,7 @@ __global__ __launch_bounds__(256) void attention_combine_kernel(AttArgs a) {
 #pragma unroll 4
         for (int k = g; k < a.splits; k += 8) {
             const float w = wt[k];
-            if (w > 0.f) {                                         // a split without keys left its sums unwritten
+            if (!(w < 0.f)) {                                      // (a weight that vanished takes part: 0 times NaN is NaN)
                 const f32x4 o = *reinterpret_cast<const f32x4*>(a.part + (k * rows + row) * a.D + c);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) s[j] += w * o[j];
@@ -263,19 +268,19 @@ __global__ __launch_bounds__(256) void attention_combine_kernel(AttArgs a) {
     }
     *reinterpret_cast<f32x4*>(&red[g][c]) = s;
     __syncthreads();
-    const float inv = l > 0.f ? 1.f / l : 0.f;
+    const float inv = 1.f / l;                                     // of scores that are all -inf: 0 / 0
     if (threadIdx.x < a.D) {
         float t = 0.f;
 #pragma unroll
         for (int k = 0; k < 8; ++k) t += red[k][threadIdx.x];
-        ((T*)a.out)[row * a.D + threadIdx.x] = (T)(t * inv);
+        ((T*)a.out)[row * a.D + threadIdx.x] = (T)(none ? 0.f : t * inv);
     }
     if (a.lse && threadIdx.x == 0) {
         const int h = (int)(row % a.H);
         const long long bn = row / a.H;
         const int n = (int)(bn % a.N);
         const long long b = bn / a.N;
-        a.lse[(b * a.H + h) * a.N + n] = l > 0.f ? (m + log2f(l)) * 0.69314718055994531f : -INFINITY;
+        a.lse[(b * a.H + h) * a.N + n] = none ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
     }
 }
 

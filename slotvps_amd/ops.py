@@ -1410,7 +1410,8 @@ def attention(q, k, v, q_lens=None, k_lens=None, frame=0, window=0, scale=None, 
     frame = 0: every query sees every key. frame > 0: tokens of one frame (that many tokens) see each other and all earlier frames (1: the
     causal order of single tokens), window > 0: only the last `window` frames with their own. The last query stands at the last key, so N
     new tokens attend over a memory of M >= N with the same arguments. Keys that a row does not see but that lie within its batch entry's
-    length must be finite.
+    length must be finite. Non-finite scores act as in the formula: a row that
+    sees a NaN or +inf score, or only -inf, is NaN.
     Returns out [B, N, H, D] (zeros for rows behind q_lens and rows that see nothing); with return_lse also the log-sum-exp [B, H, N] fp32
     (-inf for such rows) that attention_bwd takes. Differentiable in q, k, v. Single queries over a long memory are split over its keys."""
     q, k, v, cfg = _att_args(q, k, v, q_lens, k_lens, frame, window, scale)

@@ -650,3 +650,77 @@ def test_linear_act_short_sums_over_wide_results(cuda, c):
     check(ops.linear_act_bwd(dy, _rand((big, wide), BF, 75, cuda), w, want_dw=False)[0], dy, w.t())
     dy, x = _rand((c, big), BF, 76, cuda), _rand((c, wide), BF, 77, cuda)
     check(ops.linear_act_bwd(dy, x, _rand((big, wide), BF, 78, cuda), want_dx=False)[1], dy.t(), x.t())
+
+
+# ---- values that are not finite -----------------------------------------------------------------------------------------------
+
+NONFINITE = [  # B, N, M, H, Hk, D, frame
+    (2, 70, 90, 4, 2, 64, 0),                                       # few keys: the statistics' own products
+    (2, 150, 200, 4, 2, 128, 0),
+    (2, 200, 200, 2, 1, 40, 1),
+    (2, 1, 3000, 4, 2, 128, 0),                                     # the keys are split
+    (2, 9, 2500, 6, 2, 32, 1),
+]
+
+
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("case", NONFINITE)
+@pytest.mark.parametrize("kind", ["nan key", "infinite key", "infinite query", "nan value"])
+def test_attention_of_visible_values_that_are_not_finite(cuda, dt, case, kind):
+    """A row that sees a score (or a value) that is not finite is NaN, as its softmax is; rows of other entries and key heads do not change."""
+    B, N, M, H, Hk, D, frame = case
+    G = H // Hk
+    q, k, v, do = _rand((B, N, H, D), dt, 1, cuda), _rand((B, M, Hk, D), dt, 2, cuda), _rand((B, M, Hk, D), dt, 3, cuda), _rand((B, N, H, D), dt, 4, cuda)
+    ref, tol = _attention_ref(q, k, v, do, [N] * B, [M] * B, frame, 0, D ** -0.5, dt)
+    at = max(M - max(N // 2, 1), 0)                                  # seen by about half of the rows in order, by all without
+    hit = torch.zeros((B, N, H), dtype=torch.bool, device=cuda)
+    if kind == "infinite query":
+        q[1, N - 1, 1, 3] = math.inf                                 # products of either sign: inf - inf, or a maximum of inf
+        hit[1, N - 1, 1] = True
+    else:
+        (v if kind == "nan value" else k)[1, at, 0, 5] = math.inf if kind == "infinite key" else math.nan
+        hit[1, :, :G] = _visible(N, M, N, M, frame, 0, cuda)[:, at, None]
+    if kind == "infinite key":                                       # a score of -inf has no weight, one of +inf is the row's maximum
+        hit &= (q[..., 5] > 0)
+    out, lse = ops.attention(q, k, v, frame=frame, return_lse=True)
+    got = torch.isnan(out.float()).any(-1)
+    if kind == "nan value":                                          # in order it may reach rows that do not see it: 0 times NaN
+        assert torch.isfinite(lse).all() and (got.equal(hit) if not frame else got[hit].all())
+    else:
+        assert got.equal(hit) and torch.isnan(out.float()).all(-1).equal(hit), "out"
+        assert torch.isnan(lse.transpose(1, 2)).equal(hit), "lse"
+    away = torch.ones((B, H), dtype=torch.bool, device=cuda)         # (entry, head) pairs that have nothing to do with it
+    away[1, :G] = False
+    pick = lambda t: t.transpose(1, 2)[away]
+    _close(pick(out), pick(ref[0]), pick(tol[0]), "out elsewhere")
+    dq, dk, dv = ops.attention_bwd(do, q, k, v, out, lse, frame=frame)
+    _close(pick(dq), pick(ref[2]), pick(tol[1]), "dq elsewhere")
+    for t, r, e, name in ((dk, ref[3], tol[2], "dk elsewhere"), (dv, ref[4], tol[3], "dv elsewhere")):
+        # fp16: e's share of the result's own rounding vanishes with |dk|, the rounding itself stays half of 2^-24 below 2^-14
+        _close(torch.cat([t[0], t[1, :, 1:]], 1), torch.cat([r[0], r[1, :, 1:]], 1), torch.cat([e[0], e[1, :, 1:]], 1) + _sub(dt), name)
+    assert torch.isnan(dq.float()).any(-1)[hit].all(), "dq"
+    if kind != "nan value":                                          # their weights are NaN, and so is what these weights carry to the keys they see
+        seen = (_visible(N, M, N, M, frame, 0, cuda) & hit[1, :, :G].any(1)[:, None]).any(0)
+        assert torch.isnan(dv[1, :, 0].float()).all(-1)[seen].all(), "dv"
+
+
+@pytest.mark.parametrize("N,M", [(70, 90), (1, 3000)])
+def test_attention_of_rows_whose_scores_are_all_minus_infinity_or_very_low(cuda, N, M):
+    """A row whose visible scores are all -inf has no softmax (0 / 0), which is not a row that sees nothing. Scores of -2^29 (far below any
+    16-bit mask value) are a softmax like any other: equal ones give the mean of the values."""
+    q, k, v = (torch.zeros((1, n, 1, 16), dtype=BF, device=cuda) for n in (N, M, M))
+    v.copy_(_rand(v.shape, BF, 3, cuda))
+    k[..., 0], q[..., 0] = 2.0 ** 16, -2.0 ** 13
+    out, lse = ops.attention(q, k, v, return_lse=True, scale=1.0)
+    mean = v.double().mean(1, keepdim=True).expand_as(out)
+    _close(out, mean, 2.0 ** -8 * mean.abs() + 2.0 ** -7 * v.double().abs().mean(1, keepdim=True), "mean")
+    # base 2 and back: two roundings of a number of 2^30
+    assert (lse.double() / -2.0 ** 29 - 1).abs().max() < 2.0 ** -22
+    k[..., 0] = 1
+    q.zero_()
+    q[:, 0, :, 0] = -math.inf
+    out, lse = ops.attention(q, k, v, return_lse=True)
+    assert torch.isnan(out[:, 0].float()).all() and torch.isfinite(out[:, 1:].float()).all()
+    assert not torch.isfinite(lse[:, :, 0]).any()
+    dq, dk, dv = ops.attention_bwd(torch.ones_like(out), q, k, v, out, lse)
+    assert torch.isnan(dq[:, 0].float()).any() and torch.isnan(dv.float()).all()
