@@ -236,6 +236,12 @@ __device__ __forceinline__ void att_dq(const AttArgs& a, const int id, char* sme
     }
     AttArgsMem& m = *att_args();
     if (n >= m.N) return;
+    if (lo >= hi) {                                                // behind qlen, or sees nothing: its weights are 0, but 0 times a key that is NaN is not
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[db][i] = 0.f;
+    }
     const long long orow = ((long long)b * m.N + n) * m.H + hk * m.G + (row - n * m.G);
     if (m.splits > 1) {
         float* po = m.part + (split * ((long long)m.B * m.N * m.H) + orow) * m.D;
@@ -246,6 +252,23 @@ __device__ __forceinline__ void att_dq(const AttArgs& a, const int id, char* sme
     T* o = (T*)m.dq + orow * m.D;
 #pragma unroll
     for (int db = 0; db < DB; ++db) att_store_block<T>(o, 32 * db, h, m.D, acc[db], m.scale);
+}
+
+// tokens [n0, n1) that see a key of [k0, k1): their frame is not before the first key's, and not `window` or more behind the last key's
+template <typename A>
+__device__ __forceinline__ void att_seen_by(const A& a, int k0, int k1, int qlen, int klen, int& n0, int& n1) {
+    n0 = 0;
+    n1 = k0 < klen ? qlen : 0;
+    if (a.frame > 0 && n1 > 0) {
+        k1 = k1 < klen ? k1 : klen;
+        const long long off = (long long)klen - qlen;
+        const long long first = (long long)(k0 / a.frame) * a.frame - off;
+        if (first > 0) n0 = first < qlen ? (int)first : qlen;
+        if (a.window > 0) {
+            const long long last = ((long long)((k1 - 1) / a.frame) + a.window) * a.frame - off;
+            if (last < n1) n1 = last > 0 ? (int)last : 0;
+        }
+    }
 }
 
 // dK, dV of 128 keys: a wave owns 32 keys, their k and v stay in registers as operand fragments (at DP = 128 the sums and they are 192 of 256
@@ -264,18 +287,8 @@ __device__ __forceinline__ void att_dkdv(const AttArgs& a, const int id, char* s
     const int qlen = att_qlen(a, b), klen = att_klen(a, b);
     const int wk0 = t * 128, k0 = wk0 + 32 * w, key = k0 + r;
 
-    // tokens that see a key of [wk0, wk1): their frame is not before the first key's, and not `window` or more behind the last key's
-    int n0 = 0, n1 = wk0 < klen ? qlen : 0;
-    if (a.frame > 0 && n1 > 0) {
-        const int wk1 = wk0 + 128 < klen ? wk0 + 128 : klen;
-        const long long off = (long long)klen - qlen;
-        const long long first = (long long)(wk0 / a.frame) * a.frame - off;
-        if (first > 0) n0 = first < qlen ? (int)first : qlen;
-        if (a.window > 0) {
-            const long long last = ((long long)((wk1 - 1) / a.frame) + a.window) * a.frame - off;
-            if (last < n1) n1 = last > 0 ? (int)last : 0;
-        }
-    }
+    int n0, n1;
+    att_seen_by(a, wk0, wk0 + 128, qlen, klen, n0, n1);
     int tb = 0, te = 0;
     if (n0 < n1) {
         tb = (int)((long long)n0 * a.G / QT);
@@ -423,6 +436,13 @@ __device__ __forceinline__ void att_dkdv(const AttArgs& a, const int id, char* s
     }
     AttArgsMem& m = *att_args();
     if (key >= m.M) return;
+    att_seen_by(m, key, key + 1, qlen, klen, n0, n1);
+    if (n0 >= n1) {                                                // behind klen, or seen by no row: 0 times a row that is NaN is not 0
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) { dk[db][i] = 0.f; dv[db][i] = 0.f; }
+    }
     const long long orow = ((long long)b * m.M + key) * m.Hk + hk;
     if (m.k_splits > 1) {
         const long long rows = (long long)m.B * m.M * m.Hk;

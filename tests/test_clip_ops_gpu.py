@@ -724,3 +724,25 @@ def test_attention_of_rows_whose_scores_are_all_minus_infinity_or_very_low(cuda,
     assert not torch.isfinite(lse[:, :, 0]).any()
     dq, dk, dv = ops.attention_bwd(torch.ones_like(out), q, k, v, out, lse)
     assert torch.isnan(dq[:, 0].float()).any() and torch.isnan(dv.float()).all()
+
+
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("N,M,H,Hk,D,frame,window", [(70, 90, 4, 2, 64, 0, 0), (150, 200, 4, 2, 128, 0, 0), (200, 200, 2, 1, 40, 1, 0), (1, 3000, 4, 2, 128, 0, 0),
+                                                     (2000, 40, 4, 1, 32, 0, 0), (70, 300, 2, 2, 64, 10, 2)])
+def test_attention_gradients_behind_the_lengths_are_zero_beside_values_that_are_not_finite(cuda, dt, N, M, H, Hk, D, frame, window):
+    """Rows and keys behind the lengths, rows that see nothing and keys that no row sees have zero outputs and gradients, also where others are NaN."""
+    B = 3
+    ql, kl = [N, max(N - 37, 0), max(N - 5, 1)], [M - 33, M, M // 2]
+    base = [_rand((B, N, H, D), dt, 1, cuda), _rand((B, M, Hk, D), dt, 2, cuda), _rand((B, M, Hk, D), dt, 3, cuda), _rand((B, N, H, D), dt, 4, cuda)]
+    kw = dict(q_lens=_lens(ql, B, N, cuda), k_lens=_lens(kl, B, M, cuda), frame=frame, window=window)
+    for which in range(4):                                           # a NaN in q, k, v, dO
+        x = [t.clone() for t in base]
+        x[which][:, 0] = math.nan
+        out, lse = ops.attention(*x[:3], return_lse=True, **kw)
+        dq, dk, dv = ops.attention_bwd(x[3], *x[:3], out, lse, **kw)
+        for b in range(B):
+            none = ~_visible(N, M, ql[b], kl[b], frame, window, cuda)
+            row, key = none.all(1), none.all(0)
+            assert not out[b, row].any() and torch.isneginf(lse[b][:, row]).all(), (which, b)
+            assert not dq[b, row].any(), (which, b)
+            assert not dk[b, key].any() and not dv[b, key].any(), (which, b)
