@@ -562,7 +562,7 @@ int svps_mask_decode_f32_fwd(const float* feat, const float* embed, const float*
  *
  * svps_linear_act_fwd: y = act(x W^T + bias) + residual; x [M, K] (row stride ldx), W [N, K] (row stride ldw), bias [N] (bias_f32: fp32,
  *   else of `dtype`; NULL: none), residual [M, N] contiguous or NULL, act 0 none, 1 ReLU, 2 GELU (erf), y [M, N] contiguous, gate [M, N]
- *   contiguous int16 or NULL: act' at the same place in units of 2^-14, for the backward call. fp32 sums, one rounding. bf16 / fp16.
+ *   contiguous int16 or NULL: act' at the same place in units of 2^-14 (-32768: NaN), for the backward call. fp32 sums, one rounding. bf16 / fp16.
  * svps_linear_act_bwd: dz = dy * gate (gate NULL: dz = dy), dx = dz W, dW = dz^T x, db = column sums of dz; dx / dw / db may be NULL.
  *   dy [M, N] (row stride ldy), gate contiguous; db fp32 (db_f32) or of `dtype`.
  * *_workspace_bytes: `unaligned` nonzero if any of the row-strided tensors does not start on 16 bytes. Workspaces start on 16 bytes.

@@ -111,7 +111,7 @@ __device__ __forceinline__ void lin_act(float z, float& y, float& g) {
     g = 1.f;
     if constexpr (ACT == kActRelu) {
         y = z > 0.f ? z : z != z ? z : 0.f;
-        g = z > 0.f ? 1.f : 0.f;
+        g = z > 0.f ? 1.f : z != z ? z : 0.f;
     } else if constexpr (ACT == kActGelu) {
         const float e = __builtin_amdgcn_exp2f(-0.72134752044448170f * z * z);
         const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f * 0.70710678118654752f, fabsf(z), 1.f));
@@ -125,6 +125,9 @@ __device__ __forceinline__ void lin_act(float z, float& y, float& g) {
 }
 
 constexpr float kGateOne = 16384.f;               // slopes are held as int16 in units of 2^-14 (they lie in [-0.13, 1.13]): off by 3e-5 at most
+constexpr short kGateNan = -32768;                // no slope: of a NaN
+__device__ __forceinline__ short lin_gate(float g) { return g == g ? (short)(int)rintf(g * kGateOne) : kGateNan; }
+__device__ __forceinline__ float lin_slope(short q) { return q == kGateNan ? NAN : (float)q * (1.f / kGateOne); }
 
 template <typename T>
 __device__ __forceinline__ float lin_bias(const LinArgs& a, int n) {
@@ -176,12 +179,12 @@ __device__ __forceinline__ void lin_epilogue(const LinArgs& a, int m, int n, con
             typedef short s16x8 __attribute__((ext_vector_type(8)));
             s16x8 q;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) q[j] = (short)(int)rintf(g[j] * kGateOne);
+            for (int j = 0; j < 8; ++j) q[j] = lin_gate(g[j]);
             *reinterpret_cast<s16x8*>((short*)a.gate + o) = q;
         }
     } else {
         ((T*)a.y)[o] = (T)y[0];
-        if (a.gate) ((short*)a.gate)[o] = (short)(int)rintf(g[0] * kGateOne);
+        if (a.gate) ((short*)a.gate)[o] = lin_gate(g[0]);
     }
 }
 
@@ -583,7 +586,7 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(const T* dy, long long l
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     v[j] = (float)d[u][j];
-                    if (gate) v[j] *= (float)g[u][j] * (1.f / kGateOne);
+                    if (gate) v[j] *= lin_slope(g[u][j]);
                     s[j] += v[j];
                 }
                 if (dz) *reinterpret_cast<v8*>(dz + m * ldz + c0) = att_pack<T>(v);
@@ -597,7 +600,7 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(const T* dy, long long l
                 v[j] = 0.f;
                 if (c0 + j < N) {
                     v[j] = (float)dy[(long long)m * ldy + c0 + j];
-                    if (gate) v[j] *= (float)gate[(long long)m * N + c0 + j] * (1.f / kGateOne);
+                    if (gate) v[j] *= lin_slope(gate[(long long)m * N + c0 + j]);
                 }
                 s[j] += v[j];
             }

@@ -1535,7 +1535,7 @@ def linear_act(x, weight, bias=None, act=ACT_NONE, residual=None, return_gate=Fa
     fp16, bias [N] of that type or fp32, residual [..., N], act ACT_NONE, ACT_RELU or ACT_GELU (erf). Any K >= 1 and N; widths that are
     multiples of 8 with 16-byte aligned rows are read in place, others are copied with padded rows first. fp32 sums, one rounding.
     Returns y [..., N] contiguous; with return_gate (y, gate) without an autograd graph: act' at the same place for
-    linear_act_bwd, int16 in units of 2^-14 (None for ACT_NONE).
+    linear_act_bwd, int16 in units of 2^-14, -32768 where the activation's argument is NaN (None for ACT_NONE).
     Differentiable in x, weight, bias, residual. fp32 tokens: slot_gemm / bgemm."""
     x, weight, residual = _linear_args(x, weight, bias, act, residual)
     if not return_gate and torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad) or

@@ -746,3 +746,21 @@ def test_attention_gradients_behind_the_lengths_are_zero_beside_values_that_are_
             assert not out[b, row].any() and torch.isneginf(lse[b][:, row]).all(), (which, b)
             assert not dq[b, row].any(), (which, b)
             assert not dk[b, key].any() and not dv[b, key].any(), (which, b)
+
+
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("act", [ops.ACT_RELU, ops.ACT_GELU])
+@pytest.mark.parametrize("M,K,N", [(4, 64, 64), (130, 64, 33), (300, 64, 72), (66, 712, 16), (1234, 16, 3304)])
+def test_linear_act_slope_of_a_value_that_is_not_finite(cuda, dt, act, M, K, N):
+    """A NaN in front of the activation comes back as a NaN gradient of its row; infinities have the slopes 1 and 0."""
+    x, w, dy = _rand((M, K), dt, 1, cuda), _rand((N, K), dt, 2, cuda, 0.1), _rand((M, N), dt, 3, cuda)
+    b = torch.zeros(N, dtype=F32, device=cuda)
+    x[1], b[1], b[2] = math.nan, math.inf, -math.inf
+    y, gate = ops.linear_act(x, w, b, act=act, return_gate=True)
+    rows = torch.zeros(M, dtype=torch.bool, device=cuda)
+    rows[1] = True
+    assert torch.isnan(y.float()).all(1).equal(rows) and torch.isposinf(y[~rows, 1].float()).all() and not y[~rows, 2].any()
+    assert (gate[~rows, 1] == 1 << 14).all() and (gate[~rows, 2] == 0).all()
+    x[1] = 0                                                         # the slope alone carries it on
+    dx, dw, db = ops.linear_act_bwd(dy, x, w, gate=gate, bias=b)
+    assert torch.isnan(dx.float()).all(1).equal(rows) and torch.isnan(db).all()
