@@ -764,3 +764,16 @@ def test_linear_act_slope_of_a_value_that_is_not_finite(cuda, dt, act, M, K, N):
     x[1] = 0                                                         # the slope alone carries it on
     dx, dw, db = ops.linear_act_bwd(dy, x, w, gate=gate, bias=b)
     assert torch.isnan(dx.float()).all(1).equal(rows) and torch.isnan(db).all()
+
+
+@pytest.mark.parametrize("dt", [BF, HF])
+def test_linear_act_gelu_far_below_zero(cuda, dt):
+    """z cdf(z) is tiny there but in bf16 an ordinary number: right relative to itself. Tolerance: half a step of the type, and 2^-13 for
+    the 5e-5 of the fit, 1e-5 of the exponent's fp32 roundings at z = -12 (two of a number of 104) and the products of fp32 behind them."""
+    x = torch.linspace(-12.0, -3.0, 4097, device=cuda).to(dt)[:, None]
+    w = torch.ones((1, 1), dtype=dt, device=cuda)
+    for rows in (slice(None), slice(0, 4096, 83)):                   # tiles, and few rows
+        z = x[rows].contiguous()
+        y = ops.linear_act(z, w, act=ops.ACT_GELU)
+        ref = _act64(z.double(), ops.ACT_GELU)[0]
+        _close(y, ref, (_u(dt) + 2.0 ** -13) * ref.abs() + _sub(dt), "gelu")
