@@ -9,6 +9,7 @@ import functools
 import math
 
 import torch
+import torch.autograd.forward_ad as _fwd
 
 from . import _lib
 
@@ -1128,7 +1129,7 @@ def mask_decode_f32(feat, embed, bn_scale, bn_shift, fg_scale, fg_shift):
 # ---- clip-token operators for 16-bit tokens and for training: rotary positions with several axes (csrc/rotary_axes.hip), attention with
 # ---- its gradient (csrc/attention_fwd.hip, attention_bwd.hip), dense layer with its gradient (csrc/linear_act.hip). rotary_axes, attention
 # ---- and linear_act are differentiable; the *_bwd functions are the same gradients as plain calls (no autograd graph), the form to
-# ---- capture: inside a HIP graph capture the autograd backward of these three is refused.
+# ---- capture: inside a HIP graph capture the autograd backward of these three is refused. Forward-mode tangents are refused by all.
 
 _DTYPE_CODE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _POS_CODE = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
@@ -1141,6 +1142,12 @@ def _at(t):
     return None if t is None else t.data_ptr()
 
 
+def _no_tangent(t, name):
+    """The kernels have no forward-mode derivative: a dual tensor would come back without its tangent. Without an open level: one comparison."""
+    if _fwd._current_level >= 0 and _fwd.unpack_dual(t).tangent is not None:
+        raise RuntimeError(f"{name}: carries a forward-mode tangent, which the clip-token operators do not propagate")
+
+
 def _token_tensor(t, name, dtypes):
     """GPU tensor of one of `dtypes` with contiguous channels (anything else of that kind is copied)."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
@@ -1148,6 +1155,7 @@ def _token_tensor(t, name, dtypes):
                            "there is no CPU fallback")
     if t.dtype not in dtypes:
         raise TypeError(f"{name}: expected one of {', '.join(str(d) for d in dtypes)}, got {t.dtype}")
+    _no_tangent(t, name)
     return t if t.dim() == 0 or t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
@@ -1369,6 +1377,7 @@ def _att_bwd(dout, q, k, v, out, lse, q_lens, k_lens, frame, window, scale):
     dout = _att_tensor(dout, "dout", q.dtype)
     out = _att_tensor(out, "out", q.dtype).contiguous()
     _need(lse, "lse", torch.float32, 3)
+    _no_tangent(lse, "lse")
     if dout.shape != q.shape or out.shape != q.shape or lse.shape != (B, H, N):
         raise ValueError(f"attention_bwd: dout {tuple(dout.shape)}, out {tuple(out.shape)}, lse {tuple(lse.shape)} do not belong to q {tuple(q.shape)}")
     empty = B == 0 or N == 0 or M == 0
@@ -1462,6 +1471,7 @@ def _linear_args(x, weight, bias, act, residual):
         if not isinstance(bias, torch.Tensor) or bias.dtype not in (x.dtype, torch.float32):
             raise TypeError(f"bias: expected {x.dtype} or torch.float32")
         _need(bias, "bias", bias.dtype, 1)
+        _no_tangent(bias, "bias")
         if bias.shape[0] != N:
             raise ValueError(f"linear_act: bias must have {N} values")
     if residual is not None:

@@ -777,3 +777,25 @@ def test_linear_act_gelu_far_below_zero(cuda, dt):
         y = ops.linear_act(z, w, act=ops.ACT_GELU)
         ref = _act64(z.double(), ops.ACT_GELU)[0]
         _close(y, ref, (_u(dt) + 2.0 ** -13) * ref.abs() + _sub(dt), "gelu")
+
+
+def test_forward_mode_tangents_are_refused(cuda):
+    """The operators have no forward-mode derivative: a dual tensor is refused, not answered without its tangent."""
+    import torch.autograd.forward_ad as fw
+    x, w = _rand((4, 64), BF, 1, cuda), _rand((64, 64), BF, 2, cuda)
+    q, b = x.view(1, 4, 2, 32), torch.zeros(64, dtype=F32, device=cuda)
+    pos = torch.zeros((4, 1), device=cuda)
+    out, lse = ops.attention(q, q, q, return_lse=True)
+    with fw.dual_level():
+        d = lambda t: fw.make_dual(t, torch.ones_like(t))
+        for call in (lambda: ops.linear_act(d(x), w), lambda: ops.linear_act(x, d(w)), lambda: ops.linear_act(x, w, d(b)),
+                     lambda: ops.linear_act(x, w, residual=d(x)), lambda: ops.linear_act_bwd(d(x), x, w), lambda: ops.linear_act_bwd(x, x, w, bias=d(b)),
+                     lambda: ops.attention(d(q), q, q), lambda: ops.attention(q, d(q), q), lambda: ops.attention(q, q, d(q)),
+                     lambda: ops.attention_bwd(d(q), q, q, q, out, lse), lambda: ops.attention_bwd(q, q, q, q, out, d(lse)),
+                     lambda: ops.rotary_axes(d(q), pos, (4,)), lambda: ops.rotary_axes(q, pos, (4,), also=d(q)),
+                     lambda: ops.rotary_axes(q, d(pos), (4,)), lambda: ops.rotary_axes_bwd(d(q), pos, (4,))):
+            with pytest.raises(RuntimeError, match="tangent"):
+                call()
+            with pytest.raises(RuntimeError, match="tangent"), torch.no_grad():
+                call()
+        assert torch.equal(ops.linear_act(x, w), ops.linear_act(x.clone(), w))      # plain tensors inside a level
