@@ -15,7 +15,7 @@ import math
 import pytest
 import torch
 
-from slotvps_amd import ops
+from slotvps_amd import _lib, ops
 
 pytestmark = pytest.mark.gpu
 BF, HF, F32 = torch.bfloat16, torch.float16, torch.float32
@@ -799,3 +799,91 @@ def test_forward_mode_tangents_are_refused(cuda):
             with pytest.raises(RuntimeError, match="tangent"), torch.no_grad():
                 call()
         assert torch.equal(ops.linear_act(x, w), ops.linear_act(x.clone(), w))      # plain tensors inside a level
+
+
+# ---- every tile, split and row-block variant ----------------------------------------------------------------------------------
+
+def _linear_plan(M, N, K, cus):
+    """The library's choice of tile and split, restated: a case below that no longer reaches its variant fails instead of testing another."""
+    best, steps = None, (K + 63) // 64
+    for tile, fit, full, alone, fixed in ((256, 1, 1.5, 1.5, 6.0), (128, 2, 0.68, 0.9, 4.0), (64, 4, 0.36, 0.6, 3.0)):
+        tiles = -(-M // tile) * -(-N // tile)
+        for s in range(1, 33):
+            if s > 1 and steps // s < 4:
+                break
+            rest, depth = tiles * s % (cus * fit), float((steps + s - 1) // s)
+            one = lambda on: depth * max(on * full, alone) + fixed
+            t = tiles * s // (cus * fit) * one(fit) + (one((rest + cus - 1) // cus) if rest else 0.0) + (4.0 + s * M * N * 8.0 / 4e6 if s > 1 else 0.0)
+            if best is None or t < best[0]:
+                best = (t, tile, s)
+    return best[1:]
+
+
+VARIANTS = [  # M, K, N, act, bias, residual, (tile, split) of y, dx, dW; 0: any
+    (17, 1096, 331, ops.ACT_GELU, True, True, 0, 0, 0),             # few rows: two and four blocks of 16, more than one pass over k
+    (32, 2056, 72, ops.ACT_RELU, True, False, 0, 0, 0),
+    (33, 40, 130, ops.ACT_GELU, True, True, 0, 0, 0),
+    (64, 1100, 128, ops.ACT_GELU, False, True, 0, 0, 0),
+    (1234, 136, 3304, ops.ACT_GELU, True, True, (128, False), 0, 0),
+    (1233, 136, 3301, ops.ACT_GELU, True, True, (128, False), 0, 0),
+    (1746, 69, 4104, ops.ACT_GELU, True, True, (128, False), 0, (128, True)),
+    (73, 1744, 4264, ops.ACT_GELU, True, True, (128, True), 0, (128, False)),
+    (1155, 3424, 16, ops.ACT_GELU, True, False, 0, (128, False), 0),
+    (2389, 65, 3967, ops.ACT_GELU, True, True, (256, False), (128, True), 0),
+    (6332, 136, 4488, ops.ACT_GELU, True, True, (256, False), (128, True), (256, True)),
+    (4096, 2048, 4096, ops.ACT_RELU, True, True, (256, False), (128, False), (128, False)),
+    (66, 2728, 2960, ops.ACT_GELU, True, True, 0, 0, (256, False)),
+    (6697, 4238, 129, ops.ACT_GELU, True, True, (256, True), (256, False), (128, True)),
+    (5631, 140, 4971, ops.ACT_GELU, True, False, 0, (256, True), (128, True)),
+]
+
+
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("case", VARIANTS)
+def test_linear_act_variants(cuda, dt, case):
+    M, K, N = case[:3]
+    cus = torch.cuda.get_device_properties(cuda).multi_processor_count
+    for want, size in zip(case[6:], ((M, N, K), (M, K, N), (N, K, M))):
+        if want:
+            tile, s = _linear_plan(*size, cus)
+            assert (tile, s > 1) == want
+    tile, s = _linear_plan(M, N, K, cus)
+    packed = 2 * (M + N) * (K + 7 & ~7) if K % 8 else 0
+    parts = 4 * s * M * (N + 7 & ~7) if s > 1 and M > 64 else 0
+    assert 0 <= _lib.load().svps_linear_act_workspace_bytes(M, K, N, K, K, 0) - packed - parts < 3 * 256
+    test_linear_act_forward_and_gradients(cuda, dt, case[:6])
+
+
+@pytest.mark.parametrize("dt,G,D,N,M,frame,window", [
+    (BF, 2, 128, 250, 203, 0, 0), (HF, 2, 128, 250, 203, 1, 0), (BF, 3, 72, 171, 190, 1, 0), (HF, 3, 96, 171, 90, 0, 0), (BF, 3, 128, 171, 203, 50, 2),
+    (HF, 5, 128, 103, 120, 1, 7)])
+def test_attention_of_two_row_blocks_per_wave(cuda, dt, G, D, N, M, frame, window):
+    """Heads above 64 with workgroups of 256 rows for four rounds of the compute units, lengths that end inside them, group sizes that divide no tile."""
+    B, Hk = 32, 16
+    H = G * Hk
+    assert B * Hk * -(-N * G // 256) >= 4 * torch.cuda.get_device_properties(cuda).multi_processor_count
+    ql, kl = [N - 3 * b for b in range(B)], [M - 2 * b for b in range(B)]
+    q, k, v, do = _rand((B, N, H, D), dt, 1, cuda), _rand((B, M, Hk, D), dt, 2, cuda), _rand((B, M, Hk, D), dt, 3, cuda), _rand((B, N, H, D), dt, 4, cuda)
+    for b in range(B):
+        q[b, ql[b]:], do[b, ql[b]:], k[b, kl[b]:], v[b, kl[b]:] = math.nan, math.inf, math.nan, -math.inf
+    kw = dict(q_lens=_lens(ql, B, N, cuda), k_lens=_lens(kl, B, M, cuda), frame=frame, window=window)
+    out, lse = ops.attention(q, k, v, return_lse=True, **kw)
+    some = [0, 1, 7, B - 1]                                          # entries that are compared
+    part = lambda t: t[some]
+    ref, tol = _attention_ref(part(q), part(k), part(v), part(do), [ql[b] for b in some], [kl[b] for b in some], frame, window, D ** -0.5, dt)
+    _close(part(out), ref[0], tol[0], "out")
+    none = torch.isinf(ref[1])
+    assert torch.equal(torch.isinf(part(lse)), none) and (part(lse).double() - ref[1])[~none].abs().max() < 1e-3
+    for name, a, r, t in zip(("dq", "dk", "dv"), ops.attention_bwd(do, q, k, v, out, lse, **kw), ref[2:], tol[1:]):
+        _close(part(a), r, t, name)
+    for b in some:                                                   # alone, an entry runs in another variant: equal but for the order of its fp32 sums
+        one = ops.attention(q[b:b + 1], k[b:b + 1], v[b:b + 1], q_lens=kw["q_lens"][b:b + 1], k_lens=kw["k_lens"][b:b + 1], frame=frame, window=window)
+        _close(one, ref[0][some.index(b)][None], tol[0][some.index(b)][None], "alone")
+
+
+def test_attention_of_eight_waves_in_fp16(cuda):
+    B, N, M, H, Hk, D = 32, 250, 203, 16, 8, 64
+    q, k, v = _rand((B, N, H, D), HF, 1, cuda), _rand((B, M, Hk, D), HF, 2, cuda), _rand((B, M, Hk, D), HF, 3, cuda)
+    out = ops.attention(q, k, v, frame=1)
+    ref, tol = _attention_ref(q[:2], k[:2], v[:2], None, [N] * 2, [M] * 2, 1, 0, D ** -0.5, HF)
+    _close(out[:2], ref[0], tol[0], "out")
