@@ -9,19 +9,22 @@
 // changes the result, or write every dS to memory (2 bytes per visible pair and head).
 // Few tiles on either side: the walked range is split over workgroups that leave fp32 partial sums, added by att_add_kernel.
 //
-// P and dS are rounded to 16 bits once each, as operands of the products with dO, Q and K: beside the roundings of q, k, v and of the result
-// they make a gradient 1.4 times as far off as its own rounding. Everything else is fp32.
+// P and dS are rounded to 16 bits once each, as operands of the products with dO, Q and K (the matrix instructions take 16 bits): beside the
+// roundings of q, k, v and of the result they make a gradient 1.4 times as far off as its own rounding. Everything else is fp32. lse in fp32 is
+// off by 2^-24 of itself, which every p of the row inherits: at scores of 10^4 2e-3, at 10^6 a fifth.
 //
 // Bound: the matrix products (10 D flop per visible pair, 14 D executed). Measured in bf16, all launches, flop counted as 10 D: 4 x 4096
-// tokens, 16 heads of 128 1.84 ms = 747 TFLOP/s, causal over 4 key heads 0.97 ms = 707; 10240 tokens, 8 heads of 64 0.88 ms = 610, of 32
-// 0.54 ms = 497 TFLOP/s; 5 x 100 tokens, 8 heads of 32 10.4 us.
+// tokens, 16 heads of 128 1.75 ms = 785 TFLOP/s, causal over 4 key heads 0.96 ms = 717; 10240 tokens, 8 heads of 64 0.84 ms = 637, of 32
+// 0.52 ms = 517 TFLOP/s; 5 x 100 tokens, 8 heads of 32 10.2 us. 4 x 4096 tokens, 16 heads of 40 1.15 ms, of 72 1.87 ms, of 96 1.95 ms.
 #include "attention.h"
 #include "../../include/slotvps_hip.h"
 
 namespace svps {
 
-// A wave takes 32 packed rows. delta = sum_d dO_id O_id is O's rounding to 16 bits away from sum_j p_ij dP_ij, which the rows of many keys do
-// not notice (dS's own rounding is larger). Rows of few keys do: dS = P * (dP - delta) is then a small difference, of a single visible key
+// A wave takes 32 packed rows. delta = sum_d dO_id O_id is O's rounding to 16 bits away from sum_j p_ij dP_ij. Rows that spread over many keys do
+// not notice (dS's own rounding is larger). Rows with nearly all their weight on one of many keys notice some: dQ is off by 1.4 times its own
+// rounding at scores of standard deviation 1, by 2.2 at 4, by 3.5 at 16 (1000 tokens, 4 heads of 64); a delta from the products would cost two more
+// products over all keys. Rows of few keys notice most: dS = P * (dP - delta) is then a small difference, of a single visible key
 // zero (18 x 7 causal tokens, 2 / 1 heads of 96, against 64 bits: dQ 2.2 times as far off as its own rounding, as below 1.4 times). Where all keys
 // that a wave's rows see lie within kStatKeys, delta is therefore the second sum (over the sum of p), from the same products that dQ and dK repeat.
 constexpr int kStatKeys = 64;

@@ -6,9 +6,13 @@
 // workgroups that leave unnormalised sums with their maximum, joined by attention_combine_kernel.
 //
 // Bound: the matrix products (4 D flop per visible pair) and the softmax beside them - at heads of 128 about 40 vector instructions and 16
-// exponentials for 8 products of 32 x 32 x 16, at heads of 32 as many for 4. Measured in bf16: 4 x 4096 tokens, 16 heads of 128 557 us =
-// 985 TFLOP/s, causal 302 us = 911 TFLOP/s; 10240 tokens, 8 heads of 64 286 us = 750, of 32 215 us = 500 TFLOP/s. A single query over a long
-// memory is bound by its bytes: 5 x up to 16383 keys, 4 heads of 128 24 us = 7 TB/s.
+// exponentials for 8 products of 32 x 32 x 16, at heads of 32 as many for 4. Measured in bf16: 4 x 4096 tokens, 16 heads of 128 528 us =
+// 1041 TFLOP/s, causal 294 us = 934 TFLOP/s; 10240 tokens, 8 heads of 64 271 us = 792, of 32 204 us = 526 TFLOP/s. A single query over a long
+// memory is bound by its bytes: 5 x up to 16383 keys (126 MB in all), 4 heads of 128 23.4 us = 5.4 TB/s. Head sizes between are multiplied as
+// the next of 32, 64 and 128 and staged by per-lane addresses: 4 x 4096 tokens, 16 heads of 40 311 us, of 72 546 us, of 96 560 us.
+//
+// Scores in base 2 (scale log2 e q k) hold to 2^30 in magnitude: a score is compared with the row's reference point in one fused multiply-add,
+// whose exact result is up to the rounding of that point away from 0 - beyond 2^31 more than exp2 can take, the row becomes NaN.
 #include "attention.h"
 #include "../../include/slotvps_hip.h"
 

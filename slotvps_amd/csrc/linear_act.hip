@@ -6,7 +6,9 @@
 // ([k][m]): forward (contiguous, contiguous), dx (contiguous, k-major), dW (k-major, k-major). Fragments of a k-contiguous tile are 16-byte
 // LDS reads, of a k-major tile two hardware-transposed reads. Sums are fp32; bias, activation, slope and residual act on them before the
 // one rounding of y. The slope g is stored instead of the pre-activation: held as int16 in units of 2^-14 it is off by 3e-5 (a 16-bit
-// pre-activation in bf16: by up to 4e-3 times the curvature), and the backward pass needs no transcendental.
+// pre-activation in bf16: by up to 4e-3 times the curvature), and the backward pass needs no transcendental. That is absolute: a slope below
+// 2^-7 is coarser than bf16's own rounding, below 2^-4 than fp16's, and GELU's below z = -4.7 is held as 0. dz is rounded to 16 bits once, as an
+// operand of both products: with an activation dx and dW are 1.4 times as far off as their own rounding, without one dz is dy itself.
 //
 // Tile BM x BN x 64, WM x WN waves; operand tiles come by 16-byte LDS-DMA, the next ones while this one is multiplied. The W fragment is the
 // MFMA's row operand: a lane owns one row m and four consecutive n per accumulator quad. Tiles behind each other in memory go to one XCD (its L2
@@ -15,8 +17,8 @@
 // Operands whose rows do not start on 16 bytes or whose length is no multiple of 8 are first copied with zero-padded rows (linear_pack).
 //
 // Bound: matrix instructions, from about 1000 columns on; they run at the clock that the power allows (8192 cubed with operands of zeros:
-// 600 us). Measured in bf16: 8192 cubed 805 us = 1365 TFLOP/s, dx 820 us, dW 855 us; 10240 x 6144 -> 1536 165 us = 1170 TFLOP/s. Narrower ones
-// by their bytes and the epilogue: 32768 x 384 -> 1536 58 us, with GELU 78 us (12 vector and 2 transcendental instructions per value, which
+// 600 us). Measured in bf16: 8192 cubed 786 us = 1399 TFLOP/s, dx 824 us, dW 861 us; 10240 x 6144 -> 1536 146 us = 1325 TFLOP/s. Narrower ones
+// by their bytes and the epilogue: 32768 x 384 -> 1536 61 us, with GELU 80 us (13 vector and 2 transcendental instructions per value, which
 // with one workgroup per CU nothing runs under). A few rows by the latency of one pass over the weights.
 #include <type_traits>
 
@@ -555,8 +557,8 @@ __global__ __launch_bounds__(256) void linear_pack_kernel(LinPack a) {
 
 // dz = dy * gate (stored with row stride ldz, zero padded; skipped when dz is null) and the column sums of dz over a chunk of rows.
 // Workgroup: CT threads x 8 columns of 256 / CT rows at a time, four rows per thread in flight. CT = 32 (512 bytes of a row) for many rows;
-// CT = 4 for few, where 32-column workgroups are what fills the chip and the one chunk's sums are db (500 x 2048: 16 us wide, 7 us narrow;
-// 10240 x 1536: 7 us wide, 14 us narrow).
+// CT = 4 for few, where 32-column workgroups are what fills the chip and the one chunk's sums are db (dz and sums of 500 x 2048: 7.5 us wide,
+// 5.9 us narrow; of 10240 x 1536: 19 us wide, 78 us narrow).
 template <typename T, int CT>
 __global__ __launch_bounds__(256) void linear_dz_kernel(const T* dy, long long ldy, const short* gate, T* dz, int ldz, float* sums, void* db, int db_f32,
                                                         int M, int N, int rows_per) {
@@ -650,8 +652,9 @@ struct LinPlan { int tile, splits; size_t part_bytes; };
 // Tile (256, 128 or 64 square; one, two and four workgroups of them fit a CU) and split of the k range, by a model of the time in
 // microseconds. Measured at k = 8192: a 64-deep step of a full CU takes 1.5, 0.68 and 0.36 per workgroup on it, of a workgroup alone on
 // its CU 1.5, 0.9 and 0.6; start and epilogue 6, 4 and 3; a split's partial sums go to memory and back at 4 TB/s and cost a launch.
-// (8192 cubed: 256 gives 810 us, 128 1170 us; 500 x 256 -> 2048: 128 12 us, 64 8.6 us; dW of 32768 rows, 384 -> 1536: 64 without split
-// 242 us, 128 with 14 parts 69 us.)
+// (8192 cubed: 256 gives 778 us, 128 1045 us; 500 x 256 -> 2048 with GELU: 256 20 us, 128 8.8 us, 64 5.0 us; dW of 32768 rows, 384 -> 1536: 64
+// without split 239 us, 128 with 14 parts 67.5 us, 256 with 21 parts, which it takes, 66 us; 32768 x 384 -> 1536 with GELU: 256, which it takes,
+// 72 and 80 us on two cards, 128 72 and 76 us.)
 static LinPlan linear_plan(int M, int N, int K) {
     static const int tile[3] = {256, 128, 64}, fit[3] = {1, 2, 4};
     static const double full[3] = {1.5, 0.68, 0.36}, alone[3] = {1.5, 0.9, 0.6}, fixed[3] = {6.0, 4.0, 3.0};
@@ -705,6 +708,9 @@ static int linear_pack(const void* src, long long ld, void* dst, int rows, const
     return (int)hipGetLastError();
 }
 
+// Up to here one launch without a workspace (linear_few_kernel). Against tiles of 64, in us: 256 -> 2048: 17 rows 2.5 / 3.7, 64 rows 3.6 / 3.8;
+// 1536 -> 1536: 32 rows 6.0 / 7.0, 64 rows 9.0 / 7.8; 6144 -> 1536: 17 rows 14.3 / 9.8, 64 rows 28.8 / 12.1. The bound looks at the rows alone
+// and so is too high for sums of thousands.
 constexpr int kFewRows = 64;
 
 static bool linear_shape_ok(int M, int K, int N, long long ldx, long long ldw) {

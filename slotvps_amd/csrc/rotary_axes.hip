@@ -11,7 +11,8 @@
 // Bound: bandwidth (each value read once, written once; 6 operations per pair). A workgroup takes a few tokens: the cosines and sines of
 // their pairs once, into LDS, then all heads of both tensors as a stream of 16-byte pieces, consecutive lanes on consecutive pieces (a lane
 // per pair of pieces with the heads in a loop reads the same bytes in 96-byte shreds: 40960 tokens, 20 heads of 128: 143 us against 90 us = 4.7 TB/s). The
-// other half of a pair is a second read of a line that the wave has just asked for. Few tokens: the heads are dealt over grid.y.
+// other half of a pair is a second read of a line that the wave has just asked for. Few tokens: the heads are dealt over grid.y. fp32: 163 us =
+// 5.1 TB/s. Rows that are not aligned and sections that end inside a piece go by single elements, one in flight: at R = 40 302 us = 1.4 TB/s.
 #include "common.h"
 #include "../../include/slotvps_hip.h"
 
